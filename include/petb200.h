@@ -204,6 +204,59 @@ int petb200_softmax_run(petb200_ctx *ctx, const float *x, float *y, size_t rows,
 int petb200_attention_supported(int m, int n, int kd, int d);
 int petb200_attention_run(petb200_ctx *ctx, const float *q, const float *k, const float *v, float *out, int bs, int m, int n,
                           int kd, int d, const long long *strides, petb200_stream stream);
+/* ---- a paged cache of keys and values, and the attentions that read it (no counterpart in the reference, whose attention is the
+ * chain of operators above) ------------------------------------------------------------------------------------------
+ * A cache is two pools of pages, one for keys and one for values: element (page, slot, head, d) lies at
+ * page * k_page + slot * k_slot + head * k_head + d (strides in elements).  `dim` is a multiple of 8 up to 128; the pools and all
+ * strides are multiples of 16 bytes; anything else is PETB200_ERR_UNSUPPORTED. */
+enum { PETB200_F32 = 0, PETB200_F16 = 1, PETB200_BF16 = 2 };
+typedef struct {
+    void *k, *v;
+    long long k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int dtype, pages, page_size, heads, dim;
+} petb200_kv_cache;
+/* The sequences of one call.  Key j of sequence b lies in page page_table[b * table_stride + j / page_size], slot j % page_size.
+ * kv_lens[b] counts its keys with those of the tokens of this call, which are its last ones.  q_starts (seqs + 1 entries) gives its
+ * tokens as rows [q_starts[b], q_starts[b + 1]); NULL: every sequence has tokens / seqs of them.  The three arrays live on the device and are
+ * read when the kernels run.  Table entries past a sequence's keys are not read.  A page outside the cache counts as zeros, keys past the
+ * table's width are left out, and petb200_check_device_status reports either. */
+typedef struct {
+    const int *page_table, *kv_lens, *q_starts;
+    long long table_stride;
+    int table_width, seqs, tokens;
+} petb200_kv_seqs;
+/* Rows of a call: element (token, head, d) at token * tok + head * head_stride + d. */
+typedef struct {
+    void *p;
+    long long tok, head;
+} petb200_kv_rows;
+/* Writes the tokens' keys and values to their places in the cache, keys turned by their positions, and the turned queries to q_out.
+ * Token i of n of sequence b has position p = kv_lens[b] - n + i; pair j of the first `rotary` values of a head (values j and
+ * j + rotary / 2, or 2 j and 2 j + 1 where `interleaved`) is turned by the angle (pos0 + p) * inv_freq[j], formed in 64 bits.
+ * inv_freq NULL or rotary 0: nothing is turned.  Sources are of type src_dtype (the cache's, or PETB200_F32), rounded once to the cache's;
+ * q_out is of the cache's type.  q.p NULL: keys and values alone.  Rows outside all sequences, and tokens with p < 0, write nothing to
+ * the cache; rows outside all sequences leave q_out as it was.  A page that two sequences of the call both append to is left undefined. */
+int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, petb200_kv_rows k,
+                          petb200_kv_rows v, petb200_kv_rows q, petb200_kv_rows q_out, int q_heads, int src_dtype,
+                          const float *inv_freq, int rotary, int interleaved, int pos0, petb200_stream stream);
+/* out[token, head] = sum_j softmax_j(scale q . k_j) v_j over the token's sequence, query head `head` on key head
+ * head / (q_heads / heads).  causal: token i of n sees keys j <= kv_lens[b] - n + i, else all kv_lens[b].  A row that sees no key
+ * gives zeros; rows outside all sequences are left as they were; masked and absent keys never contribute, whatever they hold.
+ * q and out are of the cache's type, rows 16-byte aligned, and must not overlap; scores, softmax and sums are fp32 (F32 caches: products error-compensated TF32;
+ * 16-bit caches: probabilities rounded to the cache's type).  `workspace` is device memory of the size that
+ * petb200_attention_paged_workspace gives for the same call (prefix_len 0), used until the launches have run. */
+int petb200_attention_paged_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, petb200_kv_rows q,
+                                petb200_kv_rows out, int q_heads, int causal, float scale, void *workspace, size_t workspace_bytes,
+                                petb200_stream stream);
+/* The same where every sequence begins with the prefix_len keys that lie in the pages prefix_table[0 .. ceil(prefix_len / page_size)):
+ * kv_lens counts a sequence's own keys, which follow them, and every token sees the whole prefix.  Single tokens and short runs of
+ * them read the prefix once for the whole batch. */
+int petb200_attention_prefix_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const int *prefix_table,
+                                 int prefix_len, petb200_kv_rows q, petb200_kv_rows out, int q_heads, int causal, float scale,
+                                 void *workspace, size_t workspace_bytes, petb200_stream stream);
+int petb200_attention_paged_workspace(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, int prefix_len,
+                                      int q_heads, size_t *bytes);
+
 /* SoftmaxOp over any axis (the operator carries one, ref: include/operator.h:1887-1938; the reference's emitted kernel
  * only serves the last): x viewed as [outer, len, inner], normalised over len.  inner == 1 is petb200_softmax_run. */
 int petb200_softmax_axis_run(petb200_ctx *ctx, const float *x, float *y, size_t outer, int len, size_t inner,

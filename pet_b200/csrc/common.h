@@ -59,6 +59,7 @@ struct petb200_ctx {
     };
     std::vector<BandTcPlan> band_tc;
     void (*band_tc_destroy)(void *) = nullptr;
+    std::vector<const void *> smem_raised; // kernels whose shared-memory limit raise_smem() has set on this device
     ~petb200_ctx() {
         for (void *p : band_retired)
             cudaFree(p);
@@ -97,6 +98,16 @@ inline int fail(petb200_ctx *ctx, int status, const char *fmt, ...) {
             return petb200::fail((ctx), PETB200_ERR_CUDA, "%s failed: %s (%s:%d)", #call,                    \
                                  cudaGetErrorString(e_), __FILE__, __LINE__);                                \
     } while (0)
+
+// Lets `kernel` be launched with that much dynamic shared memory on the context's device (once; the call itself costs a microsecond).
+inline int raise_smem(petb200_ctx *ctx, const void *kernel, int bytes) {
+    for (const void *k : ctx->smem_raised)
+        if (k == kernel)
+            return PETB200_OK;
+    PETB200_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    ctx->smem_raised.push_back(kernel);
+    return PETB200_OK;
+}
 
 // Records a launch and converts a launch error into a status.
 inline int launched(petb200_ctx *ctx, const char *what) {

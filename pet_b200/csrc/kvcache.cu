@@ -1,0 +1,368 @@
+// A paged cache of keys and values: appending to it, and the checks and choices in front of the attentions that read it.
+//
+// k_kv_append: out = x turned by its position, pair (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin), and copied to its place.  One pass
+// over the data; bound by HBM for prompts, by latency for single tokens.  The angle of a pair is the same for every
+// head, so a block first forms the cosines and sines of its tokens in shared memory and then walks the heads in 16-byte pieces.
+// Angles: position * frequency in 64 bits, whole turns taken off there (an fp32 product at position 10^5 is off by
+// 4 * 10^-3 radians), sincospif of what is left.  The rotation itself is fp32, rounded once to the cache's type.
+#include "paged.cuh"
+#include <algorithm>
+#include <cmath>
+
+namespace petb200 {
+namespace {
+
+constexpr int kAppendThreads = 256, kAppendTokens = 4;
+
+struct AppendArgs {
+    PagedSeqs s;
+    const void *x[3];                // queries, keys, values
+    void *y[3];                      // where they go: q_out, and the two pools
+    long long x_tok[3], x_head[3];   // strides in elements
+    long long y_tok, y_head[3];      // q_out: token and head; pools: head
+    long long y_page[3], y_slot[3];
+    int heads[3], dim, rot, interleaved, pos0, tokens_per_block, vec;
+    const float *inv_freq;
+};
+
+// Eight values as floats; `vec`: the rows are on the 16-byte grid.
+template <typename S> __device__ __forceinline__ void load8(const S *p, bool vec, float (&v)[8]) {
+    if (vec) {
+        uint4 w[sizeof(S) / 2];
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(S) / 2; ++i)
+            w[i] = __ldg(reinterpret_cast<const uint4 *>(p) + i);
+        const S *e = reinterpret_cast<const S *>(w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = to_f32(e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = to_f32(p[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
+    uint4 w[sizeof(T) / 2];
+    T *e = reinterpret_cast<T *>(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        e[i] = from_f32<T>(v[i]);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+        reinterpret_cast<uint4 *>(p)[i] = w[i];
+}
+
+template <typename S, typename T> __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a) {
+    pdl_prologue();
+    __shared__ float2 turn[kAppendTokens][kPagedMaxDim / 2]; // {cos, sin}
+    __shared__ int where[kAppendTokens][3];                  // page (-1: nowhere), slot, whether the row belongs to a sequence
+    __shared__ int position[kAppendTokens];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tok0 = blockIdx.x * a.tokens_per_block, ntok = min(a.tokens_per_block, a.s.tokens - tok0);
+    if (warp < ntok) {
+        const int t = tok0 + warp;
+        int b;
+        if (a.s.q_starts) { // the last sequence that begins at or before t: as many as do, all looked at together
+            int n = 0;
+            for (int i = lane; i <= a.s.seqs; i += 32)
+                n += __ldg(a.s.q_starts + i) <= t;
+            b = (int)__reduce_add_sync(0xffffffffu, n) - 1;
+        } else
+            b = t / a.s.q_len;
+        if (lane == 0) {
+            int page = -1, slot = 0, in = 0, p = 0, t0 = 0;
+            if (b >= 0 && b < a.s.seqs) {
+                const int n = a.s.span(b, t0);
+                if (t >= t0 && t < t0 + n) {
+                    in = 1;
+                    p = __ldg(a.s.kv_lens + b) - n + (t - t0);
+                    if (p >= 0 && a.s.page_of(p) < a.s.width)
+                        page = a.s.page(b, p, slot);
+                    else if (p >= 0)
+                        atomicOr(a.s.status, kStatusPage);
+                }
+            }
+            where[warp][0] = page, where[warp][1] = slot, where[warp][2] = in;
+            position[warp] = p;
+        }
+    }
+    __syncthreads();
+    const int half = a.rot / 2;
+    for (int i = threadIdx.x; i < ntok * half; i += kAppendThreads) {
+        const int t = i / half, j = i - t * half;
+        const double turns = ((double)a.pos0 + (double)position[t]) * (double)__ldg(a.inv_freq + j) * 0.15915494309189533577; // 1 / (2 pi)
+        float sn, cs;
+        sincospif(2.f * (float)(turns - rint(turns)), &sn, &cs);
+        turn[t][j] = make_float2(cs, sn);
+    }
+    __syncthreads();
+    const int per_head = a.dim / 8, heads = a.heads[0] + a.heads[1] + a.heads[2], pieces = heads * per_head;
+    for (int i = blockIdx.y * kAppendThreads + threadIdx.x; i < ntok * pieces; i += gridDim.y * kAppendThreads) {
+        const int t = i / pieces, r = i - t * pieces, hh = r / per_head, d = (r - hh * per_head) * 8;
+        const int kind = hh < a.heads[0] ? 0 : hh < a.heads[0] + a.heads[1] ? 1 : 2;
+        const int h = hh - (kind > 0 ? a.heads[0] : 0) - (kind > 1 ? a.heads[1] : 0);
+        const int page = where[t][0];
+        if (kind ? page < 0 : !where[t][2])
+            continue;
+        const S *x = (const S *)a.x[kind] + (long long)(tok0 + t) * a.x_tok[kind] + (long long)h * a.x_head[kind];
+        float v[8];
+        load8(x + d, a.vec, v);
+        if (kind < 2 && d < a.rot) {
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2)
+                    if (d + e < a.rot) {
+                        const float2 c = turn[t][(d + e) >> 1];
+                        const float x1 = v[e], x2 = v[e + 1];
+                        v[e] = x1 * c.x - x2 * c.y, v[e + 1] = x2 * c.x + x1 * c.y;
+                    }
+            } else if ((half & 7) == 0) { // the other halves of the pairs are a piece too
+                float o[8];
+                const bool low = d < half;
+                load8(x + (low ? d + half : d - half), a.vec, o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float2 c = turn[t][low ? d + e : d + e - half];
+                    v[e] = low ? v[e] * c.x - o[e] * c.y : v[e] * c.x + o[e] * c.y;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (d + e < a.rot) {
+                        const bool low = d + e < half;
+                        const float2 c = turn[t][low ? d + e : d + e - half];
+                        const float o = to_f32(x[low ? d + e + half : d + e - half]);
+                        v[e] = low ? v[e] * c.x - o * c.y : v[e] * c.x + o * c.y;
+                    }
+            }
+        }
+        T *y = (T *)a.y[kind] + (long long)h * a.y_head[kind] + d;
+        y += kind ? (long long)page * a.y_page[kind] + (long long)where[t][1] * a.y_slot[kind] : (long long)(tok0 + t) * a.y_tok;
+        store8(y, v);
+    }
+}
+
+template <typename S, typename T> int append_launch(petb200_ctx *ctx, AppendArgs &a, cudaStream_t s) {
+    const int pieces = (a.heads[0] + a.heads[1] + a.heads[2]) * (a.dim / 8);
+    // Several tokens to a block share its angles and barriers; few tokens are spread over blocks instead, one piece a thread.
+    a.tokens_per_block = a.s.tokens >= kAppendTokens * 2 * ctx->sm_count ? kAppendTokens : 1;
+    const int blocks = ceil_div(a.s.tokens, a.tokens_per_block);
+    const int split = blocks < 4 * ctx->sm_count ? std::min(ceil_div(pieces, kAppendThreads), 64) : 1;
+    launch_pdl(k_kv_append<S, T>, dim3((unsigned)blocks, (unsigned)split), kAppendThreads, 0, s, a);
+    return launched(ctx, "k_kv_append");
+}
+
+int type_size(int dtype) { return dtype == PETB200_F32 ? 4 : 2; }
+bool on_grid(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+// Restores the calling thread's device: a call is made on the context's, whichever is current.
+struct DeviceGuard {
+    int was = -1;
+    bool moved = false;
+    explicit DeviceGuard(int device) {
+        if (cudaGetDevice(&was) == cudaSuccess && was != device)
+            moved = cudaSetDevice(device) == cudaSuccess;
+    }
+    ~DeviceGuard() {
+        if (moved)
+            (void)cudaSetDevice(was);
+    }
+};
+
+int check_cache(petb200_ctx *ctx, const char *what, const petb200_kv_cache *c, const petb200_kv_seqs *s) {
+    if (!c || !s)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
+    if (c->dtype < PETB200_F32 || c->dtype > PETB200_BF16)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: unknown type %d", what, c->dtype);
+    if (c->pages < 0 || c->page_size <= 0 || c->heads <= 0 || c->dim <= 0 || s->seqs < 0 || s->tokens < 0 || s->table_width < 0)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: a size is negative or zero", what);
+    if (c->dim % 8 || c->dim > kPagedMaxDim)
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: head widths are multiples of 8 up to %d (got %d)", what, kPagedMaxDim, c->dim);
+    const long long e = 16 / type_size(c->dtype);
+    if (!on_grid(c->k) || !on_grid(c->v) || c->k_page % e || c->k_slot % e || c->k_head % e || c->v_page % e || c->v_slot % e || c->v_head % e)
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: the pools and their strides must be multiples of 16 bytes", what);
+    if (c->k_page < 0 || c->k_slot < 0 || c->k_head < 0 || c->v_page < 0 || c->v_slot < 0 || c->v_head < 0 || s->table_stride < 0)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: negative strides", what);
+    if ((long long)s->table_width * c->page_size > 0x7fff0000ll)
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: a table row of %d pages of %d keys: more than 2^31 keys", what, s->table_width, c->page_size);
+    if (s->seqs && s->tokens) {
+        if ((s->table_width && !s->page_table) || !s->kv_lens)
+            return fail(ctx, PETB200_ERR_INVALID, "%s: no page table or no lengths", what);
+        if (c->pages && (!c->k || !c->v))
+            return fail(ctx, PETB200_ERR_INVALID, "%s: no cache", what);
+        if (!s->q_starts && s->tokens % s->seqs)
+            return fail(ctx, PETB200_ERR_INVALID, "%s: %d tokens are not the same number for each of %d sequences", what, s->tokens, s->seqs);
+    }
+    return PETB200_OK;
+}
+
+PagedSeqs device_seqs(petb200_ctx *ctx, const petb200_kv_cache *c, const petb200_kv_seqs *s) {
+    PagedSeqs d;
+    d.table = s->page_table, d.tstride = s->table_stride, d.width = s->table_width;
+    d.kv_lens = s->kv_lens, d.q_starts = s->q_starts, d.seqs = s->seqs, d.tokens = s->tokens;
+    d.q_len = s->seqs ? s->tokens / s->seqs : 0;
+    d.page_size = c->page_size, d.pages = c->pages, d.status = ctx->d_status;
+    d.page_shift = -1;
+    if ((c->page_size & (c->page_size - 1)) == 0)
+        for (d.page_shift = 0; (1 << d.page_shift) < c->page_size;)
+            ++d.page_shift;
+    return d;
+}
+
+PagedArgs attention_args(petb200_ctx *ctx, const petb200_kv_cache *c, const petb200_kv_seqs *s, int q_heads) {
+    PagedArgs a;
+    a.s = device_seqs(ctx, c, s);
+    a.kc = c->k, a.vc = c->v;
+    a.kp = c->k_page, a.ks = c->k_slot, a.kh = c->k_head, a.vp = c->v_page, a.vs = c->v_slot, a.vh = c->v_head;
+    a.hkv = c->heads, a.group = q_heads / c->heads, a.dim = c->dim;
+    return a;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Attention over the sequences' own keys behind `prefix_len` shared ones, or (a.q == nullptr) the workspace that it takes.
+int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, int prefix_len, char *ws, size_t ws_bytes, size_t *need, cudaStream_t s) {
+    const long long rows = (long long)a.s.tokens * a.group;
+    a.s.table0 = prefix_table;
+    a.s.n0 = prefix_len;
+    // A sequence with rows enough to fill a tile by itself gains nothing from the others: its keys are read as one run.
+    const bool together = prefix_len > 0 && a.s.seqs > 1 && rows / a.s.seqs < 64;
+    if (!together)
+        return paged_rows_run(ctx, dtype, a, ws, ws_bytes, need, 0, s);
+    const int dp = a.dim > 64 ? 128 : 64;
+    PagedArgs p = a; // all tokens as one sequence that has the shared keys alone
+    p.s.kv_lens = nullptr, p.s.q_starts = nullptr;
+    const long long tiles = (rows + 15) / 16 * a.hkv;
+    const int pieces = (int)std::max(1ll, std::min({(2ll * ctx->sm_count + tiles - 1) / tiles, (prefix_len + 255ll) / 256, 64ll}));
+    const size_t po = align256((size_t)pieces * a.hkv * rows * dp * 4), pml = align256((size_t)pieces * a.hkv * rows * 8);
+    p.po = a.po = reinterpret_cast<float *>(ws);
+    p.pml = a.pml = reinterpret_cast<float2 *>(ws + po);
+    size_t more = 0;
+    const bool ask = !a.q;
+    if (!ask && po + pml > ws_bytes)
+        return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes is too small", ws_bytes);
+    int rc = paged_rows_run(ctx, dtype, p, nullptr, 0, &more, pieces, s);
+    if (rc)
+        return rc;
+    a.s.n0 = 0;
+    a.pieces = pieces;
+    rc = paged_rows_run(ctx, dtype, a, ask ? nullptr : ws + po + pml, ask ? 0 : ws_bytes - po - pml, &more, 0, s);
+    *need = po + pml + more;
+    return rc;
+}
+
+int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const int *prefix_table,
+                  int prefix_len, petb200_kv_rows q, petb200_kv_rows out, int q_heads, int causal, float scale, void *workspace,
+                  size_t workspace_bytes, cudaStream_t s) {
+    if (!ctx)
+        return PETB200_ERR_INVALID;
+    if (int rc = check_cache(ctx, what, cache, seqs))
+        return rc;
+    if (q_heads <= 0 || q_heads % cache->heads)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: %d query heads on %d key heads", what, q_heads, cache->heads);
+    if (!(scale > 0.f) || !std::isfinite(scale))
+        return fail(ctx, PETB200_ERR_INVALID, "%s: the scale must be positive and finite", what);
+    if (seqs->seqs == 0 || seqs->tokens == 0)
+        return PETB200_OK;
+    if (!q.p || !out.p || (prefix_len > 0 && !prefix_table))
+        return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
+    const long long e = 16 / type_size(cache->dtype);
+    if (!on_grid(q.p) || !on_grid(out.p) || q.tok % e || q.head % e || out.tok % e || out.head % e || q.tok < 0 || q.head < 0 || out.tok < 0 || out.head < 0)
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
+    if (!on_grid(workspace))
+        return fail(ctx, PETB200_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
+    DeviceGuard guard(ctx->device);
+    PagedArgs a = attention_args(ctx, cache, seqs, q_heads);
+    a.q = q.p, a.q_tok = q.tok, a.q_head = q.head;
+    a.out = out.p, a.o_tok = out.tok, a.o_head = out.head;
+    a.causal = causal != 0;
+    a.sl2 = scale * 1.44269504088896340736f; // log2(e)
+    size_t need = 0;
+    return attend(ctx, cache->dtype, a, prefix_table, prefix_len, (char *)workspace, workspace ? workspace_bytes : 0, &need, s);
+}
+
+} // namespace
+} // namespace petb200
+
+using namespace petb200;
+
+extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, petb200_kv_rows k,
+                                     petb200_kv_rows v, petb200_kv_rows q, petb200_kv_rows q_out, int q_heads, int src_dtype,
+                                     const float *inv_freq, int rotary, int interleaved, int pos0, petb200_stream stream) {
+    const char *what = "kv_append";
+    if (!ctx)
+        return PETB200_ERR_INVALID;
+    if (int rc = check_cache(ctx, what, cache, seqs))
+        return rc;
+    if (src_dtype != cache->dtype && src_dtype != PETB200_F32)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: sources are of the cache's type or fp32", what);
+    if (!inv_freq)
+        rotary = 0;
+    if (rotary < 0 || rotary > cache->dim || rotary % 2)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: %d values of %d cannot be turned in pairs", what, rotary, cache->dim);
+    if (q_heads < 0 || (q.p && q_heads == 0))
+        return fail(ctx, PETB200_ERR_INVALID, "%s: %d query heads", what, q_heads);
+    if (seqs->seqs == 0 || seqs->tokens == 0)
+        return PETB200_OK;
+    if (!k.p || !v.p || (q.p && !q_out.p))
+        return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
+    const long long e = 16 / type_size(cache->dtype), es = 16 / type_size(src_dtype);
+    if (q.p && (!on_grid(q_out.p) || q_out.tok % e || q_out.head % e || q_out.tok < 0 || q_out.head < 0))
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q_out must start on 16-byte boundaries", what);
+    AppendArgs a{};
+    a.s = device_seqs(ctx, cache, seqs);
+    const petb200_kv_rows src[3] = {q, k, v};
+    a.vec = 1;
+    for (int i = 0; i < 3; ++i) {
+        a.heads[i] = i ? cache->heads : (q.p ? q_heads : 0);
+        a.x[i] = src[i].p, a.x_tok[i] = src[i].tok, a.x_head[i] = src[i].head;
+        if (a.heads[i] && (!on_grid(src[i].p) || src[i].tok % es || src[i].head % es))
+            a.vec = 0;
+    }
+    a.y[0] = q_out.p, a.y_tok = q_out.tok, a.y_head[0] = q_out.head;
+    a.y[1] = cache->k, a.y_page[1] = cache->k_page, a.y_slot[1] = cache->k_slot, a.y_head[1] = cache->k_head;
+    a.y[2] = cache->v, a.y_page[2] = cache->v_page, a.y_slot[2] = cache->v_slot, a.y_head[2] = cache->v_head;
+    a.dim = cache->dim, a.rot = rotary, a.interleaved = interleaved != 0, a.pos0 = pos0, a.inv_freq = inv_freq;
+    if ((long long)(a.heads[0] + a.heads[1] + a.heads[2]) * a.dim > 1 << 24)
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: a token of more than 2^24 values", what);
+    DeviceGuard guard(ctx->device);
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (cache->dtype == PETB200_F32)
+        return append_launch<float, float>(ctx, a, s);
+    if (cache->dtype == PETB200_F16)
+        return src_dtype == PETB200_F32 ? append_launch<float, __half>(ctx, a, s) : append_launch<__half, __half>(ctx, a, s);
+    return src_dtype == PETB200_F32 ? append_launch<float, __nv_bfloat16>(ctx, a, s) : append_launch<__nv_bfloat16, __nv_bfloat16>(ctx, a, s);
+}
+
+extern "C" int petb200_attention_paged_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, petb200_kv_rows q,
+                                           petb200_kv_rows out, int q_heads, int causal, float scale, void *workspace,
+                                           size_t workspace_bytes, petb200_stream stream) {
+    return attention_run(ctx, "attention_paged", cache, seqs, nullptr, 0, q, out, q_heads, causal, scale, workspace, workspace_bytes,
+                         (cudaStream_t)stream);
+}
+
+extern "C" int petb200_attention_prefix_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs,
+                                            const int *prefix_table, int prefix_len, petb200_kv_rows q, petb200_kv_rows out, int q_heads,
+                                            int causal, float scale, void *workspace, size_t workspace_bytes, petb200_stream stream) {
+    if (ctx && prefix_len < 0)
+        return fail(ctx, PETB200_ERR_INVALID, "attention_prefix: a prefix of %d keys", prefix_len);
+    return attention_run(ctx, "attention_prefix", cache, seqs, prefix_table, prefix_len, q, out, q_heads, causal, scale, workspace,
+                         workspace_bytes, (cudaStream_t)stream);
+}
+
+extern "C" int petb200_attention_paged_workspace(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, int prefix_len,
+                                                 int q_heads, size_t *bytes) {
+    if (!ctx)
+        return PETB200_ERR_INVALID;
+    if (!bytes || prefix_len < 0)
+        return fail(ctx, PETB200_ERR_INVALID, "attention_paged_workspace: bad arguments");
+    *bytes = 0;
+    if (int rc = check_cache(ctx, "attention_paged_workspace", cache, seqs))
+        return rc;
+    if (q_heads <= 0 || q_heads % cache->heads)
+        return fail(ctx, PETB200_ERR_INVALID, "attention_paged_workspace: %d query heads on %d key heads", q_heads, cache->heads);
+    if (seqs->seqs == 0 || seqs->tokens == 0)
+        return PETB200_OK;
+    return attend(ctx, cache->dtype, attention_args(ctx, cache, seqs, q_heads), nullptr, prefix_len, nullptr, 0, bytes, nullptr);
+}

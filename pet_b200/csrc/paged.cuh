@@ -1,0 +1,101 @@
+// What the kernels over a paged cache of keys and values share: how a token finds its sequence, a sequence its keys and a key
+// its page (kvcache.cu appends, paged_rows.cu and paged_tiles.cu attend).
+#pragma once
+#include "common.h"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace petb200 {
+
+constexpr int kPagedMaxDim = 128; // head widths served: multiples of 8 up to this (a row is whole 16-byte pieces)
+// Bits of the context's status word besides 1 (a wait that ran out): what the lengths and tables on the device may get wrong.
+constexpr int kStatusPage = 2; // a page outside the cache, or a sequence with more keys than its row of the table has pages for
+
+// Sequences of one call.  Lengths and tables live on the device; the host knows only how much there can be.
+struct PagedSeqs {
+    const int *table = nullptr, *table0 = nullptr; // pages of each sequence's own keys; of the keys that all of them begin with
+    long long tstride = 0;
+    const int *kv_lens = nullptr, *q_starts = nullptr;
+    int width = 0, n0 = 0, q_len = 0, seqs = 0, tokens = 0;
+    int page_size = 1, page_shift = -1, pages = 0;
+    int *status = nullptr;
+
+    // Tokens [t0, t0 + n) of sequence b.  Starts that run backwards or past the tokens give fewer tokens, never others' memory.
+    __device__ __forceinline__ int span(int b, int &t0) const {
+        if (!q_starts) {
+            t0 = b * q_len;
+            return q_len;
+        }
+        t0 = min(max(__ldg(q_starts + b), 0), tokens);
+        return min(max(__ldg(q_starts + b + 1), t0), tokens) - t0;
+    }
+    // Keys of its own that sequence b has.
+    __device__ __forceinline__ int own(int b) const {
+        if (!kv_lens)
+            return 0;
+        const int n = __ldg(kv_lens + b), most = width * page_size;
+        if (n > most)
+            atomicOr(status, kStatusPage);
+        return min(max(n, 0), most);
+    }
+    __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
+    // The page that holds key `key` of sequence b (keys [0, n0) are the shared ones), its place in `slot`; -1: not a page.
+    __device__ __forceinline__ int page(int b, int key, int &slot) const {
+        const int own_key = key - n0;
+        const int k = own_key < 0 ? key : own_key, i = page_of(k);
+        slot = k - i * page_size;
+        const int p = own_key < 0 ? __ldg(table0 + i) : __ldg(table + b * tstride + i);
+        if ((unsigned)p < (unsigned)pages)
+            return p;
+        atomicOr(status, kStatusPage);
+        return -1;
+    }
+    // Keys that token i of n sees, of n0 + own: all shared ones, and its own up to the one that came with it.
+    __device__ __forceinline__ int visible(int i, int n, int own, int causal) const {
+        return n0 + (causal ? min(max(own - n + i + 1, 0), own) : own);
+    }
+};
+
+struct PagedArgs {
+    PagedSeqs s;
+    const void *q = nullptr, *kc = nullptr, *vc = nullptr;
+    void *out = nullptr;
+    long long q_tok = 0, q_head = 0, o_tok = 0, o_head = 0; // strides in elements
+    long long kp = 0, ks = 0, kh = 0, vp = 0, vs = 0, vh = 0; // of the cache: page, slot, head
+    int hkv = 0, group = 1, dim = 0, causal = 0;
+    float sl2 = 0.f; // scale * log2(e): the softmax runs on powers of two
+    // Pieces: a row's sum over part of its keys, O unnormalised [piece][hkv][rows][DP] with {m, l} beside it, rows = tokens * group.
+    // m is the largest score * sl2; -inf: the row sees none of these keys, -FLT_MAX: it sees some, all of them at -inf.
+    float *po = nullptr;
+    float2 *pml = nullptr;
+    int pieces = 0;     // pieces written (this launch) or merged in (po / pml of an earlier launch)
+    // Split ranges of paged_rows.cu: two pieces and one descriptor per CTA.
+    float *ro = nullptr;
+    float2 *rml = nullptr;
+    int4 *meta = nullptr;
+};
+
+// fp32 values to the cache's type, rounded to nearest.
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// 16 bytes to shared memory; `bytes` 0 writes zeros and reads nothing.
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// 2^x by the hardware's approximation (2 ulp; -inf gives 0).
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+int paged_rows_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s);
+int paged_tiles_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s);
+
+} // namespace petb200

@@ -1,0 +1,673 @@
+// Attention of a few query rows over a paged cache: single tokens, draft tokens, and every call in fp32.
+//
+//   out[row] = sum_j 2^(t_j - m) v_j / sum_j 2^(t_j - m),   t_j = scale log2(e) q[row] . k_j,   m = max_j t_j
+//
+// A tile is 16 rows = (token, query head) pairs that share one key head, so a key is read once for all the heads it serves.  A CTA
+// is four warps; a step of it is 4 x CK keys, CK of them (16 halves, 8 floats) per warp, and every warp runs by itself: its
+// own ring of stages filled by its own 16-byte asynchronous copies, its own running maximum, sum and 16 x DP accumulators in
+// registers.  The warps meet once, at the end of a tile.  Bound by HBM: per 16 keys of width 128 a warp issues 32
+// mma.sync.m16n8k16 and 16 ldmatrix beside 8 KB of loads, a third of the issue slots that those 8 KB take to arrive.  (A 16-row tile
+// would leave seven eighths of a 128-row tcgen05 tile empty; paged_tiles.cu takes over where there are rows for it.)
+//
+// Work is split by ranges: the key steps of all (sequence, row tile, key head) units are laid end to end and every CTA takes an
+// equal share, whatever the lengths; a unit that crosses a border leaves one piece per CTA, and k_paged_join adds the pieces in order.
+//
+// fp32 runs on the TF32 tensor cores with both operands split in two (x = hi + lo, hi the upper 11 bits: hi hi + hi lo + lo hi,
+// 2^-21 of a product left out), and the product with V starts from zero for every 8 keys and is added in registers, since a tensor core's
+// own accumulation cuts off instead of rounding.  Scores, statistics and sums are fp32 for every type; probabilities are
+// rounded to the cache's type for the second product (16-bit types; the sum of the row takes them unrounded).
+//
+// Rows that see no key give zeros.  A masked key never contributes, whatever its value: its score is replaced before the
+// maximum, and non-finite values of its v are taken out of the stage before the product (see `scrub`).
+#include "paged.cuh"
+#include "tc_ptx.cuh"
+#include <algorithm>
+#include <cfloat>
+
+namespace petb200 {
+namespace {
+
+constexpr int kRowWarps = 4, kRowThreads = 32 * kRowWarps, kRows = 16;
+
+template <typename T, int DP> struct RowCfg {
+    static constexpr bool f32 = sizeof(T) == 4;
+    static constexpr int CK = f32 ? 8 : 16;                 // keys of a warp's step
+    static constexpr int KT = CK * kRowWarps;               // keys of a CTA's step
+    static constexpr int CPR = DP * (int)sizeof(T) / 16;    // 16-byte pieces of a row
+    static constexpr int RPI = 32 / CPR;                    // rows that one copy instruction of the warp covers
+    static constexpr int NI = CK / RPI;                     // copy instructions per operand and step
+    static constexpr int HALF = CK * DP * (int)sizeof(T);   // bytes of one operand's stage
+    static constexpr int NST = DP == 128 ? 3 : 4;           // stages
+    static constexpr int WARP_BYTES = 2 * HALF * NST;
+    static constexpr int SMEM = WARP_BYTES * kRowWarps;
+    static constexpr int CTAS = DP == 128 ? 2 : 3;          // per SM, by shared memory
+    static_assert(WARP_BYTES >= kRows * (DP + 2) * 4, "a warp's stages hold its accumulators when the warps meet");
+    static_assert(SMEM * CTAS <= 224 * 1024, "shared memory of an SM");
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T> __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo with hi the upper 11 bits of x; an infinity is all in hi.
+__device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo) {
+    hi = x & 0xffffe000u;
+    const float h = __uint_as_float(hi), f = __uint_as_float(x);
+    lo = h == f ? 0u : __float_as_uint(f - h);
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value)
+        return ptx::pack_f16x2(a, b);
+    else
+        return ptx::pack_bf16x2(a, b);
+}
+template <typename T> __device__ __forceinline__ bool finite(T v) {
+    const float f = to_f32(v);
+    return fabsf(f) <= FLT_MAX;
+}
+
+// Sum of `x` over the threads before this one, and over all of them in `total`.
+__device__ __forceinline__ unsigned block_scan(unsigned x, unsigned &total, unsigned *tmp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned inc = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
+        inc += lane >= o ? v : 0u;
+    }
+    __syncthreads(); // (tmp of an earlier scan has been read)
+    if (lane == 31)
+        tmp[warp] = inc;
+    __syncthreads();
+    unsigned before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+        before += w < warp ? tmp[w] : 0u;
+        total += tmp[w];
+    }
+    return before + inc - x;
+}
+
+enum { kModeRanges = 0, kModeUnits = 1, kModePieces = 2 };
+
+// One unit: rows [16 rt, 16 rt + 16) of sequence b's (token, head) pairs on key head h.
+struct Unit {
+    int b, rt, h, t0, ql, own, n; // n: keys that its last row sees
+};
+
+template <typename T, int DP> struct RowTile {
+    using C = RowCfg<T, DP>;
+    static constexpr int NJ = C::CK / 8;
+    static constexpr int QR = C::f32 ? DP / 8 * 8 : DP / 16 * 4; // registers of the query fragments (fp32: hi and lo)
+
+    float o[DP / 8][4];
+    float m[2], l[2];
+
+    __device__ __forceinline__ static int swz(int row, int piece) { return piece ^ (row & 7); }
+
+    // Issues the copies of keys [base, base + CK) of the unit; keys from `n` on are zeros.
+    __device__ __forceinline__ static void fetch(const PagedArgs &a, const Unit &u, uint32_t stage, int base, int n) {
+        const int lane = threadIdx.x & 31;
+        long long ko = -1, vo = 0;
+        if (lane < C::CK && base + lane < n) {
+            int slot;
+            const int p = a.s.page(u.b, base + lane, slot);
+            if (p >= 0) {
+                ko = (long long)p * a.kp + (long long)slot * a.ks + (long long)u.h * a.kh;
+                vo = (long long)p * a.vp + (long long)slot * a.vs + (long long)u.h * a.vh;
+            }
+        }
+        const int piece = lane % C::CPR;
+        const T *kc = (const T *)a.kc, *vc = (const T *)a.vc;
+        const bool col = piece * (16 / (int)sizeof(T)) < a.dim;
+#pragma unroll
+        for (int i = 0; i < C::NI; ++i) {
+            const int row = i * C::RPI + lane / C::CPR;
+            const long long k = __shfl_sync(0xffffffffu, ko, row), v = __shfl_sync(0xffffffffu, vo, row);
+            const int bytes = col && k >= 0 ? 16 : 0;
+            const long long at = piece * (16 / (int)sizeof(T));
+            const uint32_t dst = stage + row * (DP * (int)sizeof(T)) + swz(row, piece) * 16;
+            cp_async_16_or_zero(dst, bytes ? kc + k + at : kc, bytes);
+            cp_async_16_or_zero(dst + C::HALF, bytes ? vc + v + at : vc, bytes);
+        }
+    }
+
+    // Query fragments of the tile, straight from the rows.
+    __device__ __forceinline__ static void load_q(const PagedArgs &a, const Unit &u, uint32_t (&qf)[QR]) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        const T *p[2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int row = u.rt * kRows + g + 8 * r, tok = row / a.group, hd = row - tok * a.group;
+            p[r] = tok < u.ql ? (const T *)a.q + (long long)(u.t0 + tok) * a.q_tok + (long long)(u.h * a.group + hd) * a.q_head : nullptr;
+        }
+        if constexpr (C::f32) {
+#pragma unroll
+            for (int k = 0; k < DP / 8; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { // a0 (g, c) a1 (g + 8, c) a2 (g, c + 4) a3 (g + 8, c + 4)
+                    const int d = k * 8 + c + (e >> 1) * 4;
+                    const float x = p[e & 1] && d < a.dim ? __ldg((const float *)p[e & 1] + d) : 0.f;
+                    split_tf32(__float_as_uint(x), qf[k * 8 + e], qf[k * 8 + 4 + e]);
+                }
+        } else {
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = k * 16 + 2 * c + (e >> 1) * 8;
+                    qf[k * 4 + e] = p[e & 1] && d < a.dim ? __ldg((const unsigned *)(p[e & 1] + d)) : 0u;
+                }
+        }
+    }
+
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                o[t][e] = 0.f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.f;
+    }
+
+    // Column of accumulator o[t][e] (fp32 spreads a lane's columns so that v is read 16 bytes at a time).
+    __device__ __forceinline__ static int column(int t, int e) {
+        const int c = threadIdx.x & 3;
+        return C::f32 ? (t >> 2) * 32 + 8 * c + 4 * (e & 1) + (t & 3) : t * 8 + 2 * c + (e & 1);
+    }
+
+    // Non-finite values of v in a step whose keys some rows do not see: a product with probability 0 would be NaN.  They are
+    // added where they are seen (an infinity or a NaN outlives any factor) and taken out of the stage.
+    __device__ __forceinline__ void scrub(unsigned char *vst, int base, int lim0, int lim1) {
+        const int lane = threadIdx.x & 31;
+        T *v = reinterpret_cast<T *>(vst);
+        constexpr int E = 16 / (int)sizeof(T);
+#pragma unroll 1
+        for (int r = 0; r < C::CK; ++r)
+#pragma unroll
+            for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = column(t, e);
+                    const T x = v[(r * C::CPR + swz(r, d / E)) * E + d % E];
+                    if (!finite(x)) {
+                        o[t][e] += base + r < lim0 ? to_f32(x) : 0.f;
+                        o[t][e + 2] += base + r < lim1 ? to_f32(x) : 0.f;
+                    }
+                }
+        __syncwarp();
+        for (int i = lane; i < C::CK * DP; i += 32)
+            if (!finite(v[i]))
+                v[i] = from_f32<T>(0.f);
+        __syncwarp();
+    }
+
+    // One step: keys [base, base + CK) in `stage`; row g sees keys below lim0, row g + 8 below lim1.
+    __device__ __forceinline__ void step(const PagedArgs &a, const uint32_t (&qf)[QR], uint32_t stage, unsigned char *stage_p, int base,
+                                         int lim0, int lim1, bool masked) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+        float s[NJ][4];
+        if constexpr (C::f32) {
+            float x[3][4];
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[i][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) { // two k steps of 8 per ldmatrix: pieces 4 k .. 4 k + 3 of the 8 keys
+                uint32_t r[4];
+                const int row = lane & 7;
+                ldsm4(stage + row * (DP * 4) + swz(row, 4 * k + (lane >> 3)) * 16, r);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t bh[2], bl[2];
+                    split_tf32(r[2 * h], bh[0], bl[0]);
+                    split_tf32(r[2 * h + 1], bh[1], bl[1]);
+                    uint32_t qh[4], ql[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        qh[e] = qf[(2 * k + h) * 8 + e], ql[e] = qf[(2 * k + h) * 8 + 4 + e];
+                    mma8(x[0], qh, bh[0], bh[1]);
+                    mma8(x[1], qh, bl[0], bl[1]);
+                    mma8(x[2], ql, bh[0], bh[1]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                s[0][e] = x[0][e] + (x[1][e] + x[2][e]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    s[j][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                uint32_t r[4]; // (keys 0-7, k 0-7) (0-7, 8-15) (8-15, 0-7) (8-15, 8-15)
+                const int row = (lane & 7) + ((lane >> 4) << 3);
+                ldsm4(stage + row * (DP * 2) + swz(row, 2 * k + ((lane >> 3) & 1)) * 16, r);
+                uint32_t qq[4] = {qf[4 * k], qf[4 * k + 1], qf[4 * k + 2], qf[4 * k + 3]};
+                mma16<T>(s[0], qq, r[0], r[1]);
+                mma16<T>(s[1], qq, r[2], r[3]);
+            }
+        }
+        float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[j][e] *= a.sl2, s[j][e + 2] *= a.sl2;
+                if (masked) {
+                    const int key = base + j * 8 + 2 * c + e;
+                    s[j][e] = key < lim0 ? s[j][e] : -INFINITY;
+                    s[j][e + 2] = key < lim1 ? s[j][e + 2] : -INFINITY;
+                }
+                mx0 = fmaxf(mx0, s[j][e]), mx1 = fmaxf(mx1, s[j][e + 2]);
+            }
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
+        }
+        if (__any_sync(0xffffffffu, mx0 > m[0] || mx1 > m[1])) {
+            const float n0 = fmaxf(m[0], mx0), n1 = fmaxf(m[1], mx1);
+            const float f0 = m[0] == n0 ? 1.f : exp2_approx(m[0] - n0), f1 = m[1] == n1 ? 1.f : exp2_approx(m[1] - n1);
+            m[0] = n0, m[1] = n1;
+            l[0] *= f0, l[1] *= f1;
+#pragma unroll
+            for (int t = 0; t < DP / 8; ++t)
+                o[t][0] *= f0, o[t][1] *= f0, o[t][2] *= f1, o[t][3] *= f1;
+        }
+        const float z0 = m[0] == -INFINITY ? 0.f : m[0], z1 = m[1] == -INFINITY ? 0.f : m[1]; // (nothing seen so far: every power is 0)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[j][e] = exp2_approx(s[j][e] - z0), s[j][e + 2] = exp2_approx(s[j][e + 2] - z1);
+                l[0] += s[j][e], l[1] += s[j][e + 2];
+            }
+        if (masked) {
+            bool bad = false;
+            const uint4 *v = reinterpret_cast<const uint4 *>(stage_p + C::HALF);
+            for (int i = lane; i < C::CK * C::CPR; i += 32) {
+                const uint4 w = v[i];
+                const T *x = reinterpret_cast<const T *>(&w);
+#pragma unroll
+                for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+                    bad |= !finite(x[e]);
+            }
+            if (__any_sync(0xffffffffu, bad))
+                scrub(stage_p + C::HALF, base, lim0, lim1);
+        }
+        if constexpr (C::f32) {
+            // k index c of the product is key 2 c, c + 4 is key 2 c + 1: the scores are where the product wants them
+            uint32_t ph[4], pl[4];
+            split_tf32(__float_as_uint(s[0][0]), ph[0], pl[0]);
+            split_tf32(__float_as_uint(s[0][2]), ph[1], pl[1]);
+            split_tf32(__float_as_uint(s[0][1]), ph[2], pl[2]);
+            split_tf32(__float_as_uint(s[0][3]), ph[3], pl[3]);
+            const unsigned char *vst = stage_p + C::HALF;
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) { // lane g's column of tile 4 i + e is 32 i + 4 g + e
+                const int r0 = 2 * c, r1 = 2 * c + 1;
+                const uint4 w0 = *reinterpret_cast<const uint4 *>(vst + r0 * (DP * 4) + swz(r0, 8 * i + g) * 16);
+                const uint4 w1 = *reinterpret_cast<const uint4 *>(vst + r1 * (DP * 4) + swz(r1, 8 * i + g) * 16);
+                const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t h0, l0, h1, l1;
+                    split_tf32(x0[e], h0, l0);
+                    split_tf32(x1[e], h1, l1);
+                    float y[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma8(y, pl, h0, h1);
+                    mma8(y, ph, l0, l1);
+                    mma8(y, ph, h0, h1);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+                        o[4 * i + e][z] += y[z];
+                }
+            }
+        } else {
+            const uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]), pack2<T>(s[1][2], s[1][3])};
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) {
+                uint32_t r[4]; // (keys 0-7, cols 0-7) (keys 8-15, cols 0-7) (keys 0-7, cols 8-15) (keys 8-15, cols 8-15)
+                const int row = (lane & 7) + (((lane >> 3) & 1) << 3);
+                ldsm4_t(stage + C::HALF + row * (DP * 2) + swz(row, 2 * t + (lane >> 4)) * 16, r);
+                mma16<T>(o[2 * t], p, r[0], r[1]);
+                mma16<T>(o[2 * t + 1], p, r[2], r[3]);
+            }
+        }
+    }
+};
+
+// {m, l, O} of one row from several places, in the order of the pieces.
+struct Joined {
+    float M = -INFINITY, L = 0.f;
+};
+__device__ __forceinline__ float piece_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2_approx(m - M); }
+
+template <typename T> __device__ __forceinline__ void store4(T *p, float4 v) {
+    if constexpr (sizeof(T) == 4)
+        *reinterpret_cast<float4 *>(p) = v;
+    else
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2<T>(v.x, v.y), pack2<T>(v.z, v.w));
+}
+// The row's result from its sums: zeros where it sees nothing.
+__device__ __forceinline__ float4 settle(float4 v, float M, float L) {
+    if (M == -INFINITY)
+        return make_float4(0.f, 0.f, 0.f, 0.f);
+    const float r = 1.f / L;
+    return make_float4(v.x * r, v.y * r, v.z * r, v.w * r);
+}
+__device__ __forceinline__ void fma4(float4 &x, float w, float4 y) {
+    x.x = fmaf(w, y.x, x.x), x.y = fmaf(w, y.y, x.y), x.z = fmaf(w, y.z, x.z), x.w = fmaf(w, y.w, x.w);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int mode) {
+    using C = RowCfg<T, DP>;
+    using Tile = RowTile<T, DP>;
+    pdl_prologue();
+    extern __shared__ __align__(1024) unsigned char smem[];
+    __shared__ unsigned tmp[kRowWarps];
+    __shared__ unsigned found[2]; // sequence that holds this CTA's first step, and where it begins
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    unsigned char *ring_p = smem + warp * C::WARP_BYTES;
+    const uint32_t ring = ptx::smem_u32(ring_p);
+
+    // ---- which steps are this CTA's ------------------------------------------------------------------------------
+    const bool one = a.s.kv_lens == nullptr; // all tokens against the shared keys: a single sequence without keys of its own
+    const int seqs = one ? 1 : a.s.seqs;
+    auto tokens_of = [&](int b, int &t0) {
+        if (one) {
+            t0 = 0;
+            return a.s.tokens;
+        }
+        return a.s.span(b, t0);
+    };
+    auto steps_of = [&](int b) { return mode == kModeRanges ? max(1, (a.s.n0 + a.s.own(b) + C::KT - 1) / C::KT) : 1; };
+    auto cost_of = [&](int b) -> unsigned {
+        int t0;
+        const int tiles = ceil_div(tokens_of(b, t0) * a.group, kRows);
+        return tiles ? (unsigned)(tiles * a.hkv) * (unsigned)steps_of(b) : 0u;
+    };
+    unsigned total = 0;
+    for (int b0 = 0; b0 < seqs; b0 += kRowThreads) {
+        unsigned t;
+        block_scan(b0 + (int)threadIdx.x < seqs ? cost_of(b0 + threadIdx.x) : 0u, t, tmp);
+        total += t;
+    }
+    const unsigned G = mode == kModeRanges ? min(gridDim.x, total) : total, cta = blockIdx.x;
+    if (mode == kModeRanges && threadIdx.x == 0 && a.meta)
+        a.meta[cta] = make_int4(-1, 0, 0, 0);
+    if (cta >= G)
+        return;
+    // whole units are taken from the last one down: later rows of a prompt see more keys
+    const unsigned begin = mode == kModeRanges ? (unsigned)((unsigned long long)cta * total / G) : total - 1 - cta;
+    const unsigned end = mode == kModeRanges ? (unsigned)((unsigned long long)(cta + 1) * total / G) : begin + 1;
+    unsigned run = 0;
+    for (int b0 = 0; b0 < seqs; b0 += kRowThreads) {
+        unsigned t;
+        const int b = b0 + threadIdx.x;
+        const unsigned c = b < seqs ? cost_of(b) : 0u, at = run + block_scan(c, t, tmp);
+        if (c && at <= begin && begin - at < c)
+            found[0] = b, found[1] = at;
+        run += t;
+    }
+    __syncthreads();
+    int b = found[0];
+    unsigned b_at = found[1];
+
+    for (unsigned pos = begin; pos < end;) {
+        unsigned c = cost_of(b);
+        while (pos - b_at >= c) {
+            b_at += c;
+            c = cost_of(++b);
+        }
+        const unsigned steps = steps_of(b), unit = (pos - b_at) / steps, first = (pos - b_at) - unit * steps;
+        const unsigned last = min(steps, first + (end - pos));
+        Unit u;
+        u.b = b, u.rt = unit / a.hkv, u.h = unit - u.rt * a.hkv;
+        u.ql = tokens_of(b, u.t0);
+        u.own = one ? 0 : a.s.own(b);
+        const int row_end = min((u.rt + 1) * kRows, u.ql * a.group) - 1; // last row of the tile
+        u.n = a.s.visible(row_end / a.group, u.ql, u.own, a.causal);
+        // the unit's steps of this CTA as keys
+        const int all = (u.n + C::KT - 1) / C::KT;
+        int s0 = first, s1 = min((int)last, all);
+        if (mode == kModeUnits)
+            s0 = 0, s1 = all;
+        else if (mode == kModePieces) {
+            s0 = (int)((long long)all * blockIdx.y / gridDim.y), s1 = (int)((long long)all * (blockIdx.y + 1) / gridDim.y);
+        }
+        const int r0 = u.rt * kRows + g, tok0 = r0 / a.group, tok1 = (r0 + 8) / a.group;
+        const int lim0 = tok0 < u.ql ? a.s.visible(tok0, u.ql, u.own, a.causal) : 0, lim1 = tok1 < u.ql ? a.s.visible(tok1, u.ql, u.own, a.causal) : 0;
+        const int full = a.s.visible(u.rt * kRows / a.group, u.ql, u.own, a.causal); // keys that every row sees
+
+        Tile tile;
+        tile.reset();
+        const int base0 = warp * C::CK;
+#pragma unroll
+        for (int st = 0; st < C::NST - 1; ++st) {
+            const int key = (s0 + st) * C::KT + base0;
+            if (s0 + st < s1 && key < u.n)
+                Tile::fetch(a, u, ring + st * 2 * C::HALF, key, u.n);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+        uint32_t qf[Tile::QR];
+        Tile::load_q(a, u, qf);
+        int st = 0;
+#pragma unroll 1
+        for (int i = s0; i < s1; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(C::NST - 2) : "memory");
+            __syncwarp(); // every lane's copies of this stage are in, and every lane is done with the stage that is filled next
+            {
+                const int nx = i + C::NST - 1, key = nx * C::KT + base0, to = st == 0 ? C::NST - 1 : st - 1;
+                if (nx < s1 && key < u.n)
+                    Tile::fetch(a, u, ring + to * 2 * C::HALF, key, u.n);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+            const int key = i * C::KT + base0;
+            if (key < u.n)
+                tile.step(a, qf, ring + st * 2 * C::HALF, ring_p + st * 2 * C::HALF, key, lim0, lim1, key + C::CK > full);
+            st = st == C::NST - 1 ? 0 : st + 1;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();
+
+        // ---- the warps meet: {m, l} and O of each in its own stages --------------------------------------------------
+        float *wo = reinterpret_cast<float *>(ring_p);
+        float2 *wm = reinterpret_cast<float2 *>(wo + kRows * DP);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float l = tile.l[r];
+            l += __shfl_xor_sync(0xffffffffu, l, 1);
+            l += __shfl_xor_sync(0xffffffffu, l, 2);
+            const int lim = r ? lim1 : lim0, seen = lim > s0 * C::KT + base0 && s1 > s0; // this warp's first key at least
+            if ((lane & 3) == 0)
+                wm[g + 8 * r] = make_float2(seen ? fmaxf(tile.m[r], -FLT_MAX) : -INFINITY, l);
+        }
+#pragma unroll
+        for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                wo[(g + 8 * (e >> 1)) * DP + Tile::column(t, e)] = tile.o[t][e];
+        __syncthreads();
+        {
+            const int row = threadIdx.x >> 3, part = threadIdx.x & 7, rg = u.rt * kRows + row, tok = rg / a.group, hd = rg - tok * a.group;
+            if (tok < u.ql) {
+                const bool whole = mode != kModeRanges || (first == 0 && last == steps);
+                const long long grow = (long long)(u.t0 + tok) * a.group + hd, rows = (long long)a.s.tokens * a.group;
+                const int merged = mode != kModePieces && whole ? a.pieces : 0;
+                float M = -INFINITY, L = 0.f, w[kRowWarps];
+#pragma unroll
+                for (int x = 0; x < kRowWarps; ++x) {
+                    w[x] = reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * DP * 4)[row].x;
+                    M = fmaxf(M, w[x]);
+                }
+                for (int p = 0; p < merged; ++p)
+                    M = fmaxf(M, a.pml[((long long)p * a.hkv + u.h) * rows + grow].x);
+#pragma unroll
+                for (int x = 0; x < kRowWarps; ++x) {
+                    w[x] = piece_weight(w[x], M);
+                    L += w[x] * reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * DP * 4)[row].y;
+                }
+                for (int p = 0; p < merged; ++p) {
+                    const float2 ml = a.pml[((long long)p * a.hkv + u.h) * rows + grow];
+                    L += piece_weight(ml.x, M) * ml.y;
+                }
+                const int slot = first > 0 ? 0 : 1; // of a cut unit: continued from the CTA before, or left to the one after
+                float *po = mode == kModePieces ? a.po + (((long long)blockIdx.y * a.hkv + u.h) * rows + grow) * DP
+                                                : a.ro + ((long long)(2 * cta + slot) * kRows + row) * DP;
+                if (part == 0 && mode == kModePieces)
+                    a.pml[((long long)blockIdx.y * a.hkv + u.h) * rows + grow] = make_float2(M, L);
+                else if (part == 0 && !whole)
+                    a.rml[(long long)(2 * cta + slot) * kRows + row] = make_float2(M, L);
+                T *out = (T *)a.out + (long long)(u.t0 + tok) * a.o_tok + (long long)(u.h * a.group + hd) * a.o_head;
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    const int col = j * 32 + part * 4;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int x = 0; x < kRowWarps; ++x)
+                        fma4(v, w[x], *reinterpret_cast<const float4 *>(smem + x * C::WARP_BYTES + (row * DP + col) * 4));
+                    for (int p = 0; p < merged; ++p) {
+                        const long long at = ((long long)p * a.hkv + u.h) * rows + grow;
+                        const float f = piece_weight(a.pml[at].x, M);
+                        if (f != 0.f)
+                            fma4(v, f, *reinterpret_cast<const float4 *>(a.po + at * DP + col));
+                    }
+                    if (mode == kModePieces || !whole)
+                        *reinterpret_cast<float4 *>(po + col) = v;
+                    else if (col < a.dim)
+                        store4<T>(out + col, settle(v, M, L));
+                }
+            }
+            if (mode == kModeRanges && first > 0 && threadIdx.x == 0) {
+                // The first CTA after the one in which the unit begins says where its pieces are.
+                const unsigned from = pos - first, c0 = (unsigned)(((unsigned long long)(from + 1) * G - 1) / total);
+                if (c0 + 1 == cta) {
+                    const unsigned c1 = (unsigned)(((unsigned long long)(from + steps) * G - 1) / total);
+                    a.meta[cta] = make_int4(u.b, u.rt, u.h, (int)c1);
+                }
+            }
+        }
+        __syncthreads(); // the stages are free again
+        pos += last - first;
+    }
+}
+
+// Adds the pieces of the units that ranges have cut.  A warp per row, four rows per CTA; CTA x looks after the unit that CTA x of the
+// launch before found continued from CTA x - 1, where it began.
+template <typename T, int DP> __global__ void __launch_bounds__(128) k_paged_join(const PagedArgs a) {
+    pdl_prologue();
+    const int4 d = a.meta[blockIdx.x];
+    if (d.x < 0)
+        return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 4 + warp;
+    int t0;
+    const int ql = a.s.span(d.x, t0), rg = d.y * kRows + row, tok = rg / a.group, hd = rg - tok * a.group;
+    if (tok >= ql)
+        return;
+    const int c0 = (int)blockIdx.x - 1, n = d.w - c0 + 1;
+    const long long grow = (long long)(t0 + tok) * a.group + hd, rows = (long long)a.s.tokens * a.group;
+    // The unit begins in c0's second piece; where it fills c0 whole, that CTA wrote it as second too (it began there).
+    auto place = [&](int i) { return (long long)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * kRows + row; };
+    auto shared = [&](int p) { return ((long long)p * a.hkv + d.z) * rows + grow; };
+    float M = -INFINITY, L = 0.f;
+    for (int i = lane; i < n + a.pieces; i += 32)
+        M = fmaxf(M, (i < n ? a.rml[place(i)] : a.pml[shared(i - n)]).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int col = lane * 4;
+#pragma unroll 4
+    for (int i = 0; i < n + a.pieces; ++i) {
+        const long long at = i < n ? place(i) : shared(i - n);
+        const float2 ml = i < n ? a.rml[at] : a.pml[at];
+        const float w = piece_weight(ml.x, M);
+        L += w * ml.y;
+        if (col < DP && w != 0.f)
+            fma4(v, w, *reinterpret_cast<const float4 *>((i < n ? a.ro : a.po) + at * DP + col));
+    }
+    if (col < a.dim)
+        store4<T>((T *)a.out + (long long)(t0 + tok) * a.o_tok + (long long)(d.z * a.group + hd) * a.o_head + col, settle(v, M, L));
+}
+
+template <typename T, int DP>
+int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
+    using C = RowCfg<T, DP>;
+    const bool one = a.s.kv_lens == nullptr;
+    // Row tiles there can be: a sequence's last one may be short.
+    const long long tiles = one || !a.s.q_starts ? (one ? 1ll : a.s.seqs) * (((long long)(one ? a.s.tokens : a.s.q_len) * a.group + kRows - 1) / kRows)
+                                                 : (long long)a.s.tokens * a.group / kRows + a.s.seqs;
+    const long long units = tiles * a.hkv, keys = (long long)a.s.n0 + (one ? 0 : (long long)a.s.width * a.s.page_size);
+    const long long steps = std::max(1ll, (keys + C::KT - 1) / C::KT);
+    if (keys > 0x7fff0000ll || units * steps > 0x7fff0000ll || (long long)a.s.tokens * a.group > 0x7fff0000ll)
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "attention over pages: %lld row tiles of up to %lld keys are more than one call takes", units, keys);
+    const int slots = ctx->sm_count * C::CTAS;
+    // Units as they are where there are several rounds of them: ranges would cut each in two for a gain of a part of a round.
+    const int mode = pieces_out ? kModePieces : (units >= 4ll * slots ? kModeUnits : kModeRanges);
+    const unsigned grid = (unsigned)(mode == kModeRanges ? std::min<long long>(slots, units * steps) : units);
+    size_t bytes = 0;
+    if (mode == kModeRanges) {
+        a.ro = reinterpret_cast<float *>(ws);
+        bytes = (size_t)grid * 2 * kRows * DP * 4;
+        a.rml = reinterpret_cast<float2 *>(ws + bytes);
+        bytes += (size_t)grid * 2 * kRows * 8;
+        a.meta = reinterpret_cast<int4 *>(ws + bytes);
+        bytes += (size_t)grid * 16;
+    }
+    *need = bytes;
+    if (!a.q) // (asked for the size alone)
+        return PETB200_OK;
+    if (bytes > ws_bytes)
+        return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes, %zu are needed", ws_bytes, bytes);
+    if (grid == 0)
+        return PETB200_OK;
+    if (int rc = raise_smem(ctx, (const void *)k_paged_rows<T, DP>, C::SMEM))
+        return rc;
+    launch_pdl(k_paged_rows<T, DP>, dim3(grid, (unsigned)std::max(1, pieces_out)), kRowThreads, C::SMEM, s, a, mode);
+    int rc = launched(ctx, "k_paged_rows");
+    if (rc || mode != kModeRanges)
+        return rc;
+    launch_pdl(k_paged_join<T, DP>, dim3(grid, kRows / 4), 128, 0, s, a);
+    return launched(ctx, "k_paged_join");
+}
+
+} // namespace
+
+int paged_rows_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
+    const bool wide = a.dim > 64;
+    switch (dtype) {
+    case PETB200_F16:
+        return wide ? rows_launch<__half, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s) : rows_launch<__half, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+    case PETB200_BF16:
+        return wide ? rows_launch<__nv_bfloat16, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s)
+                    : rows_launch<__nv_bfloat16, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+    default:
+        return wide ? rows_launch<float, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s) : rows_launch<float, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+    }
+}
+
+} // namespace petb200

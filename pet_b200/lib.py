@@ -22,6 +22,23 @@ class TransposeDesc(C.Structure):
     _fields_ = [("split", _i), ("factor", _i), ("ngroups", _i), ("group_sizes", _i * 8), ("flat", _i * 8)]
 
 
+_ll = C.c_longlong
+DTYPE_F32, DTYPE_F16, DTYPE_BF16 = range(3)
+
+
+class KvCache(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_page", _ll), ("k_slot", _ll), ("k_head", _ll), ("v_page", _ll), ("v_slot", _ll), ("v_head", _ll),
+                ("dtype", _i), ("pages", _i), ("page_size", _i), ("heads", _i), ("dim", _i)]
+
+
+class KvSeqs(C.Structure):
+    _fields_ = [("page_table", _vp), ("kv_lens", _vp), ("q_starts", _vp), ("table_stride", _ll), ("table_width", _i), ("seqs", _i), ("tokens", _i)]
+
+
+class KvRows(C.Structure):
+    _fields_ = [("p", _vp), ("tok", _ll), ("head", _ll)]
+
+
 SYMBOLS = {
     "petb200_ctx_create": (_i, [_i, C.POINTER(_vp)]),
     "petb200_ctx_destroy": (_i, [_vp]),
@@ -76,6 +93,10 @@ SYMBOLS = {
     "petb200_layernorm_run": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _fp, _vp]),
     "petb200_attention_supported": (_i, [_i, _i, _i, _i]),
     "petb200_attention_run": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "petb200_kv_append_run": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), KvRows, KvRows, KvRows, KvRows, _i, _i, _vp, _i, _i, _i, _vp]),
+    "petb200_attention_paged_run": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), KvRows, KvRows, _i, _i, _fp, _vp, _sz, _vp]),
+    "petb200_attention_prefix_run": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), _vp, _i, KvRows, KvRows, _i, _i, _fp, _vp, _sz, _vp]),
+    "petb200_attention_paged_workspace": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), _i, _i, C.POINTER(_sz)]),
     "petb200_matmul_splitk_noalloc": (_i, [_i] * 7 + [_vp, _vp, _vp, _vp, _i, _vp, C.c_char_p, _sz]),
     "petb200_plan_time": (_i, [_vp, _i, _i, C.POINTER(_fp), _vp]),
 }

@@ -17,6 +17,7 @@ from . import lib as L
 # declares its argument types), and the stream handle without a torch.cuda.Stream object around it.  torch has these two only
 # where it was built with CUDA; without them the module still imports (shapes, plans' arguments, the graph builders).
 _float32 = torch.float32
+_KV_TYPES = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
 _current_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
@@ -509,6 +510,132 @@ class Context:
         self.check(self.lib.petb200_attention_run(self.h, _ptr(q), _ptr(k), _ptr(v), _ptr(y), q.shape[0], q.shape[1], k.shape[1],
                                                    q.shape[2], v.shape[2], None, _stream()))
         return y
+
+    # ---- paged cache of keys and values --------------------------------------------------------------------
+    def _kv_stream(self):
+        """The current stream of the context's device (which need not be the current one)."""
+        if _raw_stream is None:
+            return torch.cuda.current_stream(self.device).cuda_stream
+        return _raw_stream(self.device.index)
+
+    def _kv_index(self, name, t, dim):
+        if t.dtype is not torch.int32 or t.dim() != dim or t.device != self.device:
+            raise L.PetError(L.ERR_INVALID, f"{name}: an int32 tensor of {dim} dimension(s) on {self.device} expected")
+        return t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+    def _kv_rows(self, name, t, heads, dim, dtypes, tokens=None):
+        if t.dim() != 3 or t.shape[2] != dim or (heads and t.shape[1] != heads) or (tokens is not None and t.shape[0] != tokens) or \
+                t.dtype not in dtypes or t.device != self.device:
+            raise L.PetError(L.ERR_INVALID, f"{name}: [{tokens if tokens is not None else 'tokens'}, {heads or 'heads'}, {dim}] of the cache's type on "
+                                            f"{self.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return t
+
+    def _kv_aligned(self, t):
+        """Rows as the kernels read them: contiguous in themselves and on the 16-byte grid (a dense copy where a view's are not)."""
+        s0, s1, s2 = t.stride()
+        size = t.element_size()
+        return t if s2 == 1 and not (t.data_ptr() | s0 * size | s1 * size) & 15 else t.clone(memory_format=torch.contiguous_format)
+
+    def _kv_call(self, tokens, k_cache, v_cache, page_table, kv_lens, q_starts):
+        """The two descriptions that every call on a cache takes; the last value holds what they point to."""
+        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype not in _KV_TYPES or v_cache.dtype is not k_cache.dtype or \
+                k_cache.device != self.device or v_cache.device != self.device:
+            raise L.PetError(L.ERR_INVALID, f"k_cache, v_cache: two [pages, page_size, heads, dim] of one type (fp32, fp16, bf16) on {self.device} expected")
+        pages, page_size, heads, dim = k_cache.shape
+        ks, vs = k_cache.stride(), v_cache.stride()
+        if ks[3] != 1 or vs[3] != 1:
+            raise L.PetError(L.ERR_UNSUPPORTED, "the values of a head must be contiguous in the cache")
+        table, lens = self._kv_index("page_table", page_table, 2), self._kv_index("kv_lens", kv_lens, 1)
+        seqs = lens.shape[0]
+        starts = None if q_starts is None else self._kv_index("q_starts", q_starts, 1)
+        if table.shape[0] != seqs or (starts is not None and starts.shape[0] != seqs + 1):
+            raise L.PetError(L.ERR_INVALID, f"{seqs} lengths take a page_table of {seqs} rows and {seqs + 1} q_starts")
+        cache = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], _KV_TYPES[k_cache.dtype],
+                          pages, page_size, heads, dim)
+        call = L.KvSeqs(table.data_ptr(), lens.data_ptr(), None if starts is None else starts.data_ptr(), table.stride(0), table.shape[1], seqs, tokens)
+        return cache, call, (table, lens, starts)
+
+    def kv_append(self, k, v, k_cache, v_cache, page_table, kv_lens, q_starts=None, q=None, q_out=None, inv_freq=None, interleaved=False, pos0=0):
+        """Writes new tokens' keys and values into a paged cache, keys turned by their positions; returns the turned queries (None without q).
+
+        k, v [tokens, heads, dim] (q [tokens, q_heads, dim]): of the cache's type, or fp32, rounded once; views of a merged projection are
+        read in place.  k_cache, v_cache [pages, page_size, heads, dim], fp32, fp16 or bf16, any page, slot and head strides that are
+        multiples of 16 bytes; dim a multiple of 8 up to 128.  page_table [seqs, width] int32: the pages of each sequence in order.  kv_lens
+        [seqs] int32: its keys, the new ones among them, which are the last.  q_starts [seqs + 1] int32: its tokens are rows
+        q_starts[b] .. q_starts[b + 1] - 1 (rows behind the last sequence write nothing); None: as many for each.
+        inv_freq [pairs] fp32: pair j is turned by (pos0 + position) * inv_freq[j], the first 2 * pairs values of a head: j with
+        j + pairs, or 2 j with 2 j + 1 (interleaved); None: nothing is turned.  No two sequences may append to one page."""
+        cache, call, hold = self._kv_call(k.shape[0], k_cache, v_cache, page_table, kv_lens, q_starts)
+        tokens, heads, dim = k.shape[0], cache.heads, cache.dim
+        types = (k_cache.dtype, _float32)
+        self._kv_rows("k", k, heads, dim, types)
+        self._kv_rows("v", v, heads, dim, (k.dtype,), tokens)
+        rows = []
+        for t in (k, v) if q is None else (k, v, self._kv_rows("q", q, 0, dim, (k.dtype,), tokens)):
+            t = t if t.stride(2) == 1 else t.contiguous()
+            rows.append((t, L.KvRows(t.data_ptr(), t.stride(0), t.stride(1))))
+        q_row = out_row = L.KvRows()
+        if q is not None:
+            q_row = rows[2][1]
+            if q_out is None:
+                q_out = torch.empty((tokens, q.shape[1], dim), device=self.device, dtype=k_cache.dtype)
+            else:
+                self._kv_rows("q_out", q_out, q.shape[1], dim, (k_cache.dtype,), tokens)
+                if q_out.stride(2) != 1:
+                    raise L.PetError(L.ERR_UNSUPPORTED, "q_out: the values of a head must be contiguous")
+            out_row = L.KvRows(q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
+        elif q_out is not None:
+            raise L.PetError(L.ERR_INVALID, "q_out without q")
+        pairs = 0
+        if inv_freq is not None:
+            if inv_freq.dtype is not _float32 or inv_freq.dim() != 1 or inv_freq.device != self.device:
+                raise L.PetError(L.ERR_INVALID, f"inv_freq: a vector of fp32 on {self.device} expected")
+            inv_freq = inv_freq.contiguous()
+            pairs = inv_freq.shape[0]
+        self.check(self.lib.petb200_kv_append_run(self.h, C.byref(cache), C.byref(call), rows[0][1], rows[1][1], q_row, out_row,
+                                                  0 if q is None else q.shape[1], _KV_TYPES[k.dtype], _ptr(inv_freq) if pairs else None, 2 * pairs,
+                                                  int(bool(interleaved)), int(pos0), self._kv_stream()))
+        return q_out
+
+    def _kv_attention(self, q, k_cache, v_cache, prefix_table, prefix_len, page_table, kv_lens, q_starts, causal, scale, out):
+        cache, call, hold = self._kv_call(q.shape[0], k_cache, v_cache, page_table, kv_lens, q_starts)
+        q = self._kv_aligned(self._kv_rows("q", q, 0, cache.dim, (k_cache.dtype,)))
+        tokens, q_heads = q.shape[0], q.shape[1]
+        if out is None:
+            out = torch.empty((tokens, q_heads, cache.dim), device=self.device, dtype=q.dtype)
+        else:
+            self._kv_rows("out", out, q_heads, cache.dim, (q.dtype,), tokens)
+            if out.stride(2) != 1:
+                raise L.PetError(L.ERR_UNSUPPORTED, "out: the values of a head must be contiguous")
+        need = C.c_size_t()
+        self.check(self.lib.petb200_attention_paged_workspace(self.h, C.byref(cache), C.byref(call), prefix_len, q_heads, C.byref(need)))
+        work = torch.empty(need.value, device=self.device, dtype=torch.uint8) if need.value else None
+        rows = L.KvRows(q.data_ptr(), q.stride(0), q.stride(1)), L.KvRows(out.data_ptr(), out.stride(0), out.stride(1))
+        tail = q_heads, int(bool(causal)), cache.dim ** -0.5 if scale is None else float(scale), _ptr(work), need.value, self._kv_stream()
+        if prefix_table is None:
+            self.check(self.lib.petb200_attention_paged_run(self.h, C.byref(cache), C.byref(call), *rows, *tail))
+        else:
+            self.check(self.lib.petb200_attention_prefix_run(self.h, C.byref(cache), C.byref(call), prefix_table.data_ptr(), prefix_len, *rows, *tail))
+        return out
+
+    def attention_paged(self, q, k_cache, v_cache, page_table, kv_lens, q_starts=None, causal=True, scale=None, out=None):
+        """softmax(scale q k^T) v of each sequence's newest tokens over its keys in a paged cache: q [tokens, q_heads, dim] -> the same shape.
+
+        Cache, page_table, kv_lens and q_starts as for kv_append (which puts the tokens' own keys there first); q_heads is a multiple of the
+        cache's heads, query head h reads key head h // (q_heads // heads).  causal: a token sees the keys up to its own; else all
+        kv_lens[b].  scale: None is dim ** -0.5.  A token that sees no key gives zeros; rows behind the last sequence are left as they
+        were (with out=None: unset).  Any page size, one token or many; lengths are read on the device, so the call can be captured."""
+        return self._kv_attention(q, k_cache, v_cache, None, 0, page_table, kv_lens, q_starts, causal, scale, out)
+
+    def attention_prefix(self, q, k_cache, v_cache, prefix_table, prefix_len, page_table, kv_lens, q_starts=None, causal=True, scale=None, out=None):
+        """attention_paged for sequences that all begin with the same `prefix_len` keys, stored once in the pages prefix_table [pages] int32:
+        kv_lens counts a sequence's own keys, which follow them (kv_append puts them there with pos0=prefix_len); every token sees the
+        whole prefix.  A batch of single tokens reads the prefix once for all."""
+        prefix_len = int(prefix_len)
+        table = self._kv_index("prefix_table", prefix_table, 1)
+        if prefix_len < 0 or prefix_len > table.shape[0] * k_cache.shape[1]:
+            raise L.PetError(L.ERR_INVALID, f"a prefix of {prefix_len} keys in {table.shape[0]} pages of {k_cache.shape[1]}")
+        return self._kv_attention(q, k_cache, v_cache, table, prefix_len, page_table, kv_lens, q_starts, causal, scale, out)
 
     def layernorm(self, x, gamma=None, beta=None, eps=1e-5):
         x, gamma, beta = _f32(x), _opt(gamma), _opt(beta)
