@@ -7,6 +7,7 @@
 // 4 * 10^-3 radians), sincospif of what is left.  The rotation itself is fp32, rounded once to the cache's type.
 #include "paged.cuh"
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 namespace petb200 {
@@ -219,6 +220,9 @@ PagedArgs attention_args(petb200_ctx *ctx, const petb200_kv_cache *c, const petb
     return a;
 }
 
+// Rows of one sequence and key head from which a 128-row tile is used, be it part full.
+constexpr int kTileFrom = 64;
+
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // Attention over the sequences' own keys behind `prefix_len` shared ones, or (a.q == nullptr) the workspace that it takes.
@@ -226,15 +230,22 @@ int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, in
     const long long rows = (long long)a.s.tokens * a.group;
     a.s.table0 = prefix_table;
     a.s.n0 = prefix_len;
-    // A sequence with rows enough to fill a tile by itself gains nothing from the others: its keys are read as one run.
-    const bool together = prefix_len > 0 && a.s.seqs > 1 && rows / a.s.seqs < 64;
-    if (!together)
-        return paged_rows_run(ctx, dtype, a, ws, ws_bytes, need, 0, s);
-    const int dp = a.dim > 64 ? 128 : 64;
+    const bool halves = dtype != PETB200_F32;
+    const bool full = rows / a.s.seqs >= kTileFrom; // a sequence's rows by themselves are enough for the tensor cores' tiles
+    // Such a sequence gains nothing from the others: its keys, shared and own, are read as one run.
+    if (prefix_len == 0 || a.s.seqs == 1 || full)
+        return halves && full ? paged_tiles_run(ctx, dtype, a, ws, ws_bytes, need, 0, s) : paged_rows_run(ctx, dtype, a, ws, ws_bytes, need, 0, s);
     PagedArgs p = a; // all tokens as one sequence that has the shared keys alone
     p.s.kv_lens = nullptr, p.s.q_starts = nullptr;
-    const long long tiles = (rows + 15) / 16 * a.hkv;
-    const int pieces = (int)std::max(1ll, std::min({(2ll * ctx->sm_count + tiles - 1) / tiles, (prefix_len + 255ll) / 256, 64ll}));
+    const bool tiles = halves && rows >= kTileFrom;
+    int pieces;
+    if (tiles)
+        pieces = paged_tiles_pieces(ctx, p);
+    else {
+        const long long units = (rows + 15) / 16 * a.hkv;
+        pieces = (int)std::max(1ll, std::min({(2ll * ctx->sm_count + units - 1) / units, (prefix_len + 255ll) / 256, 64ll}));
+    }
+    const int dp = a.dim > 64 ? 128 : 64;
     const size_t po = align256((size_t)pieces * a.hkv * rows * dp * 4), pml = align256((size_t)pieces * a.hkv * rows * 8);
     p.po = a.po = reinterpret_cast<float *>(ws);
     p.pml = a.pml = reinterpret_cast<float2 *>(ws + po);
@@ -242,7 +253,7 @@ int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, in
     const bool ask = !a.q;
     if (!ask && po + pml > ws_bytes)
         return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes is too small", ws_bytes);
-    int rc = paged_rows_run(ctx, dtype, p, nullptr, 0, &more, pieces, s);
+    int rc = tiles ? paged_tiles_run(ctx, dtype, p, nullptr, 0, &more, pieces, s) : paged_rows_run(ctx, dtype, p, nullptr, 0, &more, pieces, s);
     if (rc)
         return rc;
     a.s.n0 = 0;
@@ -261,8 +272,8 @@ int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *ca
         return rc;
     if (q_heads <= 0 || q_heads % cache->heads)
         return fail(ctx, PETB200_ERR_INVALID, "%s: %d query heads on %d key heads", what, q_heads, cache->heads);
-    if (!(scale > 0.f) || !std::isfinite(scale))
-        return fail(ctx, PETB200_ERR_INVALID, "%s: the scale must be positive and finite", what);
+    if (!std::isfinite(scale) || scale < FLT_MIN)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: the scale must be positive, finite and not denormal", what);
     if (seqs->seqs == 0 || seqs->tokens == 0)
         return PETB200_OK;
     if (!q.p || !out.p || (prefix_len > 0 && !prefix_table))

@@ -96,6 +96,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 
 int paged_rows_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s);
+// Pieces of the keys that paged_tiles_run() makes of a call by itself.
+int paged_tiles_pieces(petb200_ctx *ctx, const PagedArgs &a);
 int paged_tiles_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s);
 
 } // namespace petb200

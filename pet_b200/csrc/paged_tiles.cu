@@ -1,0 +1,546 @@
+// Attention of many query rows over a paged cache on the fifth-generation tensor cores (16-bit types): prompts, pieces of prompts,
+// and the shared prefix of a batch.
+//
+//   S = Q K^T,  P = 2^(S scale log2(e) - m),  O = sum P V,  out = O / l        (m, l: running maximum and sum of a row, fp32)
+//
+// A unit is 256 rows = (token, query head) pairs that share one key head, as two tiles of 128, against 128 keys at a time.  TMEM holds
+// both tiles' scores (fp32) and outputs, all 512 columns at head width 128; P takes its scores' place as 16-bit values and is the A operand
+// of the second product from there.  Roles: warps 0-3 and 4-7 do the softmax of a tile each (a thread owns a row), warps 8-11 fetch,
+// warp 12 issues the products.  The products of one tile run under the softmax of the other.
+//   tensor pipe  2 x (S: 128 x 128 x D, O: 128 x D x 128) = 2048 cycles per 128 keys at D = 128
+//   exponentials 2 x 16384 at 16 a cycle                  = 2048 cycles
+// The maximum moves only where a row's grows by more than 2^8 over the one in use (then O and l are scaled, by the softmax warps): the
+// sums stay within range and any m gives the same quotient.
+//
+// K and V rows come by 16-byte asynchronous copies in the 128-byte swizzle (piece c of row r at c ^ (r & 7)): the pages may have any size and
+// strides, and keys past the end arrive as zeros whatever the page holds there.  V is the second product's B operand as it
+// lies, its rows along K ("MN-major").  Per 128 keys and SM that is 64 KB, 4096 copies by four warps, an eighth of the issue slots.
+//
+// A masked key's score is replaced before the maximum.  Where some row of the unit does not see some key of a tile, the fetching warps
+// look for non-finite values of V and take them out (0 x infinity would be NaN); the rows that do see them get them back at the end.
+#include "paged.cuh"
+#include "tc_ptx.cuh"
+#include <algorithm>
+#include <cfloat>
+
+namespace petb200 {
+namespace {
+
+constexpr int kTileRows = 128, kTileKeys = 128, kTileThreads = 512;
+constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
+static_assert(256 * (kSoftmaxRegs + kOtherRegs) <= kTileThreads * 128, "more registers than the block was launched with: setmaxnreg would wait forever");
+constexpr int kLag = 2; // stages whose copies a fetching thread leaves in flight before it reports the one before them
+constexpr float kGrowth = 8.f;
+
+template <int DP> struct TileCfg {
+    static constexpr int STAGE = kTileKeys * DP * 2;
+    static constexpr int NS = DP == 128 ? 5 : 8; // stages of the ring, K and V in turn
+    static constexpr int Q = 2 * kTileRows * DP * 2;
+    static constexpr int SMEM = 1024 + Q + NS * STAGE;
+    static constexpr int CPR = DP / 8, RP = 128 / CPR, NP = 128 / RP; // pieces of a row; rows of a pass of the 128 threads; passes
+};
+static_assert(TileCfg<128>::SMEM <= 227 * 1024 - 512, "shared memory of a block");
+
+struct TileCtl {
+    uint64_t q_full, full[8], empty[8], s_full[2], p_full[2], o_full[2];
+    uint32_t tmem;
+    int abort, bad; // bad: non-finite values of V were taken out
+    int b, unit;
+};
+
+// D[tmem] (+)= A[smem] * B[smem], 16-bit inputs, fp32 accumulate; one thread issues.
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// Operand whose rows lie along K, 64 values (128 bytes) of the other extent each, in the 128-byte swizzle: blocks of 64 values are
+// `block` bytes apart, groups of eight rows 1024.
+__device__ __forceinline__ uint64_t smem_desc_mn128(uint32_t smem_addr, uint32_t block) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3ffff) >> 4);
+    d |= (uint64_t)(block >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+constexpr uint32_t kIdescBMajorMN = 1u << 16;
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (std::is_same<T, __half>::value)
+        return ptx::pack_f16x2(a, b);
+    else
+        return ptx::pack_bf16x2(a, b);
+}
+// Exponent bits all set in either half.
+template <typename T> __device__ __forceinline__ bool word_bad(uint32_t w) {
+    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return (w & e) == e || ((w >> 16) & e) == e;
+}
+template <typename T> __device__ __forceinline__ uint32_t word_clean(uint32_t w) {
+    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return ((w & e) == e ? 0u : w & 0xffffu) | (((w >> 16) & e) == e ? 0u : w & 0xffff0000u);
+}
+
+template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1) k_paged_tiles(const PagedArgs a, int splits, int to_pieces) {
+    using C = TileCfg<DP>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ TileCtl ctl;
+    unsigned char *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+    const uint32_t q_s = ptx::smem_u32(smem), ring = q_s + C::Q;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *abort_flag = &ctl.abort;
+
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(&ctl.q_full, 128);
+        for (int i = 0; i < C::NS; ++i) {
+            ptx::mbar_init(&ctl.full[i], 128);
+            ptx::mbar_init(&ctl.empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            ptx::mbar_init(&ctl.s_full[t], 1);
+            ptx::mbar_init(&ctl.p_full[t], 128);
+            ptx::mbar_init(&ctl.o_full[t], 1);
+        }
+        ctl.abort = ctl.bad = 0;
+        ctl.b = -1;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 12) {
+        ptx::tmem_alloc(&ctl.tmem, 512);
+        ptx::tmem_relinquish();
+    }
+    // A kernel that follows may start once every block of this one has come here: all that ran before this kernel is then done, and
+    // it may read what that wrote without waiting for this kernel.
+    ptx::grid_dep_wait();
+    ptx::grid_dep_launch_dependents();
+    __syncthreads();
+
+    // ---- which unit, which keys --------------------------------------------------------------------------------------------
+    const bool one = a.s.kv_lens == nullptr; // all tokens against the shared keys: a single sequence without keys of its own
+    auto tokens_of = [&](int b, int &t0) {
+        if (one) {
+            t0 = 0;
+            return a.s.tokens;
+        }
+        return a.s.span(b, t0);
+    };
+    auto units_of = [&](int b) {
+        int t0;
+        return ceil_div(tokens_of(b, t0) * a.group, 2 * kTileRows) * a.hkv;
+    };
+    const int split = blockIdx.x % splits, place = blockIdx.x / splits;
+    if (warp == 0) { // units are laid end to end and taken from the last one down: later rows of a prompt see more keys
+        const int seqs = one ? 1 : a.s.seqs;
+        unsigned total = 0;
+        for (int b0 = 0; b0 < seqs; b0 += 32)
+            total += __reduce_add_sync(0xffffffffu, b0 + lane < seqs ? (unsigned)units_of(b0 + lane) : 0u);
+        if ((unsigned)place < total) {
+            const unsigned mine = total - 1 - place;
+            unsigned run = 0;
+            for (int b0 = 0; b0 < seqs && run <= mine; b0 += 32) {
+                const unsigned c = b0 + lane < seqs ? (unsigned)units_of(b0 + lane) : 0u;
+                unsigned inc = c;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
+                    inc += lane >= o ? v : 0u;
+                }
+                const unsigned at = run + inc - c;
+                if (c && at <= mine && mine - at < c)
+                    ctl.b = b0 + lane, ctl.unit = (int)(mine - at);
+                run += __shfl_sync(0xffffffffu, inc, 31);
+            }
+        }
+    }
+    __syncthreads();
+    const uint32_t tmem = ctl.tmem;
+    const int b = ctl.b;
+    if (b >= 0) {
+        const int rt = ctl.unit / a.hkv, h = ctl.unit - rt * a.hkv, row0 = rt * 2 * kTileRows;
+        int t0;
+        const int ql = tokens_of(b, t0), own = one ? 0 : a.s.own(b), rows = min(2 * kTileRows, ql * a.group - row0);
+        const int tiles = rows > kTileRows ? 2 : 1;
+        const int n = a.s.visible((row0 + rows - 1) / a.group, ql, own, a.causal);  // keys that the last row sees
+        const int full = a.s.visible(row0 / a.group, ql, own, a.causal);            // keys that every row sees
+        const int all = (n + kTileKeys - 1) / kTileKeys;
+        const int k0 = (int)((long long)all * split / splits), k1 = (int)((long long)all * (split + 1) / splits), steps = k1 - k0;
+
+        if (warp >= 8 && warp < 12) {
+            ptx::reg_dealloc<kOtherRegs>();
+            // ---- fetch ------------------------------------------------------------------------------------------------
+            const int lt = threadIdx.x - 256, piece = lt % C::CPR, r0 = lt / C::CPR;
+            const uint32_t at0 = (uint32_t)((piece >> 3) * (kTileKeys * 128) + r0 * 128 + (((piece & 7) ^ (r0 & 7)) << 4)); // (rows of a thread agree in r & 7)
+            const bool col = piece * 8 < a.dim;
+            const T *kc = (const T *)a.kc + (long long)h * a.kh + piece * 8, *vc = (const T *)a.vc + (long long)h * a.vh + piece * 8;
+            if (steps > 0) {
+                for (int i = 0; i < tiles * C::NP; ++i) {
+                    const int r = i * C::RP + r0, tok = (row0 + r) / a.group, hd = row0 + r - tok * a.group;
+                    const bool in = col && r < rows;
+                    const T *src = (const T *)a.q + (in ? (long long)(t0 + tok) * a.q_tok + (long long)(h * a.group + hd) * a.q_head + piece * 8 : 0);
+                    cp_async_16_or_zero(q_s + (i / C::NP) * (C::Q / 2) + at0 + (i % C::NP) * (C::RP * 128), src, in ? 16 : 0);
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            }
+            int issued = steps > 0 ? 1 : 0, told = 0; // of Q, K 0, V 0, K 1, ...
+            auto tell = [&]() {                      // the oldest of them has arrived: its own copies, then everyone's
+                if (told > 0 && !(told & 1)) {
+                    const int j = k0 + told / 2 - 1, s = (told - 1) % C::NS;
+                    if ((j + 1) * kTileKeys > full) {
+                        unsigned char *p = smem + C::Q + s * C::STAGE + at0;
+#pragma unroll 1
+                        for (int i = 0; i < C::NP; ++i) {
+                            uint4 *w = reinterpret_cast<uint4 *>(p + i * (C::RP * 128));
+                            const uint4 x = *w;
+                            if (word_bad<T>(x.x) || word_bad<T>(x.y) || word_bad<T>(x.z) || word_bad<T>(x.w)) {
+                                *w = make_uint4(word_clean<T>(x.x), word_clean<T>(x.y), word_clean<T>(x.z), word_clean<T>(x.w));
+                                *(volatile int *)&ctl.bad = 1;
+                            }
+                        }
+                    }
+                }
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(told == 0 ? &ctl.q_full : &ctl.full[(told - 1) % C::NS]);
+                ++told;
+            };
+            bool ok = true;
+            for (int j = k0; j < k1 && ok; ++j) {
+                int pid[C::NP];
+#pragma unroll
+                for (int i = 0; i < C::NP; ++i) {
+                    const int key = j * kTileKeys + i * C::RP + r0;
+                    int slot;
+                    pid[i] = key < n ? a.s.page(b, key, slot) : -1;
+                }
+#pragma unroll
+                for (int v = 0; v < 2; ++v) {
+                    const int item = issued - 1, s = item % C::NS, use = item / C::NS;
+                    if (use > 0 && !ptx::mbar_try_wait(&ctl.empty[s], (use - 1) & 1)) {
+                        asm volatile("cp.async.wait_group 0;" ::: "memory"); // whoever empties the stage may be waiting for these
+                        while (told < issued)
+                            tell();
+                        ok = ok && ptx::mbar_wait(&ctl.empty[s], (use - 1) & 1, abort_flag);
+                    }
+                    if (ok) {
+                        const uint32_t dst = ring + s * C::STAGE + at0;
+                        const T *base = v ? vc : kc;
+                        const long long sp = v ? a.vp : a.kp, ss = v ? a.vs : a.ks;
+#pragma unroll
+                        for (int i = 0; i < C::NP; ++i) {
+                            const int key = j * kTileKeys + i * C::RP + r0, own_key = key < a.s.n0 ? key : key - a.s.n0;
+                            const int slot = own_key - a.s.page_of(own_key) * a.s.page_size;
+                            const bool in = col && pid[i] >= 0;
+                            cp_async_16_or_zero(dst + i * (C::RP * 128), in ? base + (long long)pid[i] * sp + (long long)slot * ss : base, in ? 16 : 0);
+                        }
+                        asm volatile("cp.async.commit_group;" ::: "memory");
+                        ++issued;
+                        if (issued - told > kLag) {
+                            asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                            tell();
+                        }
+                    }
+                }
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            while (told < issued)
+                tell();
+        } else if (warp >= 12) {
+            ptx::reg_dealloc<kOtherRegs>();
+            // ---- products ------------------------------------------------------------------------------------------------
+            if (warp == 12 && steps > 0 && ptx::elect_one()) {
+                const uint32_t kind = std::is_same<T, __half>::value ? ptx::idesc_f16(kTileRows, kTileKeys) : ptx::idesc_bf16(kTileRows, kTileKeys);
+                const uint32_t kind_o = (std::is_same<T, __half>::value ? ptx::idesc_f16(kTileRows, DP) : ptx::idesc_bf16(kTileRows, DP)) | kIdescBMajorMN;
+                auto scores = [&](int t, int s) {
+                    const uint32_t qa = q_s + t * (C::Q / 2), kb = ring + s * C::STAGE;
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t off = (k >> 2) * (kTileKeys * 128) + (k & 3) * 32;
+                        mma_f16_ss(tmem + t * 128, ptx::smem_desc_k128(qa + off), ptx::smem_desc_k128(kb + off), kind, k > 0);
+                    }
+                    ptx::mma_commit(&ctl.s_full[t]);
+                };
+                bool ok = ptx::mbar_wait(&ctl.q_full, 0, abort_flag) && ptx::mbar_wait(&ctl.full[0], 0, abort_flag);
+                if (ok) {
+                    ptx::tc_fence_after();
+                    for (int t = 0; t < tiles; ++t)
+                        scores(t, 0);
+                    ptx::mma_commit(&ctl.empty[0]);
+                }
+                for (int j = 0; j < steps && ok; ++j) {
+                    const int iv = 2 * j + 1, sv = iv % C::NS, ik = 2 * j + 2, sk = ik % C::NS;
+                    const bool more = j + 1 < steps;
+                    ok = ptx::mbar_wait(&ctl.full[sv], (iv / C::NS) & 1, abort_flag);
+                    if (ok && more)
+                        ok = ptx::mbar_wait(&ctl.full[sk], (ik / C::NS) & 1, abort_flag);
+                    for (int t = 0; t < tiles && ok; ++t) {
+                        ok = ptx::mbar_wait(&ctl.p_full[t], j & 1, abort_flag);
+                        if (!ok)
+                            break;
+                        ptx::tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < kTileKeys / 16; ++k)
+                            ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, smem_desc_mn128(ring + sv * C::STAGE + k * 2048, kTileKeys * 128),
+                                            kind_o, j > 0 || k > 0);
+                        if (more)
+                            scores(t, sk); // over P, whose product is before it in the pipe
+                        else
+                            ptx::mma_commit(&ctl.o_full[t]);
+                    }
+                    if (ok) {
+                        ptx::mma_commit(&ctl.empty[sv]);
+                        if (more)
+                            ptx::mma_commit(&ctl.empty[sk]);
+                    }
+                }
+            }
+            __syncwarp();
+        } else {
+            ptx::reg_alloc<kSoftmaxRegs>();
+            // ---- softmax: a thread owns row 32 (warp & 3) + lane of its tile ---------------------------------------------------
+            const int t = warp >> 2, r = t * kTileRows + (warp & 3) * 32 + lane, tok = (row0 + r) / a.group, hd = row0 + r - tok * a.group;
+            if (t < tiles) {
+                const bool live = r < rows;
+                const int lim = live ? a.s.visible(tok, ql, own, a.causal) : n; // (rows past the end: zeros of q, nothing is written)
+                const int warp_lim = __reduce_min_sync(0xffffffffu, lim);
+                const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
+                float m = -INFINITY, l = 0.f; // m: the maximum in use, times scale log2(e)
+                bool ok = true;
+                for (int j = 0; j < steps; ++j) {
+                    ok = ptx::mbar_wait_warp(&ctl.s_full[t], j & 1, abort_flag);
+                    if (!ok)
+                        break;
+                    ptx::tc_fence_after();
+                    uint32_t s[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        ptx::tmem_ld_32x32(s_t + c * 32, s[c]);
+                    ptx::tmem_ld_wait();
+                    const int key0 = (k0 + j) * kTileKeys;
+                    if (key0 + kTileKeys > warp_lim) {
+                        const int see = lim - key0;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                s[c][i] = c * 32 + i < see ? s[c][i] : 0xff800000u;
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        mx[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                        for (int i = 1; i < 32; ++i)
+                            mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+                    }
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
+                    if (j == 0)
+                        m = top;
+                    else if (__any_sync(0xffffffffu, top - m > kGrowth)) {
+                        // (the product with the tile before is done: its scores' successor was behind it in the pipe)
+                        const float to = fmaxf(m, top), f = m == to ? 1.f : exp2_approx(m - to);
+                        m = to;
+                        l *= f;
+#pragma unroll
+                        for (int c = 0; c < DP / 32; ++c) {
+                            uint32_t o[32];
+                            ptx::tmem_ld_32x32(o_t + c * 32, o);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            ptx::tmem_st_32x32(o_t + c * 32, o);
+                        }
+                    }
+                    const float z = m == -INFINITY ? 0.f : -m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float p = exp2_approx(fmaf(__uint_as_float(s[c][i]), a.sl2, z));
+                            sum[i & 3] += p;
+                            s[c][i] = __float_as_uint(p);
+                        }
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t p[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            p[i] = pack2<T>(__uint_as_float(s[2 * c + (i >> 4)][2 * (i & 15)]), __uint_as_float(s[2 * c + (i >> 4)][2 * (i & 15) + 1]));
+                        ptx::tmem_st_32x32(s_t + c * 32, p);
+                    }
+                    ptx::tmem_st_wait();
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(&ctl.p_full[t]);
+                }
+                // ---- the rows' results --------------------------------------------------------------------------------------
+                if (ok && steps > 0)
+                    ok = ptx::mbar_wait_warp(&ctl.o_full[t], 0, abort_flag);
+                if (ok) {
+                    ptx::tc_fence_after();
+                    const int key_a = k0 * kTileKeys, key_b = min(lim, k1 * kTileKeys);
+                    const bool seen = key_b > key_a; // this row sees some of this block's keys
+                    const long long grow = (long long)(t0 + tok) * a.group + hd, at = ((long long)split * a.hkv + h) * ((long long)a.s.tokens * a.group) + grow;
+                    const bool bad = steps > 0 && *(volatile int *)&ctl.bad;
+                    const float inv = 1.f / l;
+                    if (to_pieces && live)
+                        a.pml[at] = make_float2(seen ? fmaxf(m, -FLT_MAX) : -INFINITY, l);
+                    T *out = (T *)a.out + (long long)(t0 + tok) * a.o_tok + (long long)(h * a.group + hd) * a.o_head;
+#pragma unroll 1
+                    for (int c = 0; c < DP / 32; ++c) {
+                        uint32_t o[32];
+                        if (steps > 0) {
+                            ptx::tmem_ld_32x32(o_t + c * 32, o);
+                            ptx::tmem_ld_wait();
+                        }
+                        if (!seen) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                o[i] = 0u;
+                        }
+                        if (bad && live) {
+                            for (int key = max(key_a, full / kTileKeys * kTileKeys); key < key_b; ++key) {
+                                int slot;
+                                const int p = a.s.page(b, key, slot);
+                                const T *v = (const T *)a.vc + (long long)p * a.vp + (long long)slot * a.vs + (long long)h * a.vh + c * 32;
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float x = p >= 0 && c * 32 + i < a.dim ? to_f32(v[i]) : 0.f;
+                                    if (!(fabsf(x) <= FLT_MAX))
+                                        o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+                                }
+                            }
+                        }
+                        if (live && to_pieces) {
+                            float4 *po = reinterpret_cast<float4 *>(a.po + at * DP + c * 32);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                po[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                        } else if (live) {
+                            const float f = seen ? inv : 0.f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (c * 32 + i * 8 < a.dim) {
+                                    uint32_t w[4];
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        w[e] = pack2<T>(__uint_as_float(o[8 * i + 2 * e]) * f, __uint_as_float(o[8 * i + 2 * e + 1]) * f);
+                                    *reinterpret_cast<uint4 *>(out + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+                                }
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // ---- teardown -------------------------------------------------------------------------------------------------------------
+    if (*abort_flag) { // copies and products that may still be in flight land before the block's memory is released
+        const uint64_t t = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t < 200000ull)
+            __nanosleep(1000);
+        if (threadIdx.x == 0)
+            atomicOr(a.s.status, 1);
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 12)
+        ptx::tmem_dealloc(tmem, 512);
+}
+
+// Adds the pieces of each row: a warp per (token, head).
+template <typename T, int DP> __global__ void __launch_bounds__(128) k_paged_join_rows(const PagedArgs a) {
+    pdl_prologue();
+    const int lane = threadIdx.x & 31;
+    const long long rows = (long long)a.s.tokens * a.group, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (id >= rows * a.hkv)
+        return;
+    const int tok = (int)(id / (a.hkv * a.group)), head = (int)(id - (long long)tok * a.hkv * a.group), h = head / a.group;
+    if (a.s.q_starts) { // rows outside all sequences stay as they were
+        const int first = __ldg(a.s.q_starts), last = __ldg(a.s.q_starts + a.s.seqs);
+        if (tok < first || tok >= last)
+            return;
+    }
+    auto place = [&](int p) { return ((long long)p * a.hkv + h) * rows + (long long)tok * a.group + (head - h * a.group); };
+    float M = -INFINITY, L = 0.f;
+    for (int p = lane; p < a.pieces; p += 32)
+        M = fmaxf(M, a.pml[place(p)].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    const int col = lane * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = 0; p < a.pieces; ++p) {
+        const float2 ml = a.pml[place(p)];
+        const float w = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
+        L += w * ml.y;
+        if (col < DP && w != 0.f) {
+            const float4 y = *reinterpret_cast<const float4 *>(a.po + place(p) * DP + col);
+            v.x = fmaf(w, y.x, v.x), v.y = fmaf(w, y.y, v.y), v.z = fmaf(w, y.z, v.z), v.w = fmaf(w, y.w, v.w);
+        }
+    }
+    const float f = M == -INFINITY ? 0.f : 1.f / L;
+    if (col < a.dim)
+        *reinterpret_cast<uint2 *>((T *)a.out + (long long)tok * a.o_tok + (long long)head * a.o_head + col) =
+            make_uint2(pack2<T>(v.x * f, v.y * f), pack2<T>(v.z * f, v.w * f));
+}
+
+template <typename T, int DP>
+int tiles_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
+    using C = TileCfg<DP>;
+    const bool one = a.s.kv_lens == nullptr, even = one || !a.s.q_starts;
+    const long long rows = (long long)a.s.tokens * a.group;
+    const long long tiles = even ? (one ? 1ll : a.s.seqs) * (((long long)(one ? a.s.tokens : a.s.q_len) * a.group + 2 * kTileRows - 1) / (2 * kTileRows))
+                                 : rows / (2 * kTileRows) + a.s.seqs;
+    const long long units = tiles * a.hkv, keys = (long long)a.s.n0 + (one ? 0 : (long long)a.s.width * a.s.page_size);
+    if (keys > 0x7fff0000ll || units > 0x7fff0000ll || rows > 0x7fff0000ll)
+        return fail(ctx, PETB200_ERR_UNSUPPORTED, "attention over pages: %lld row tiles of up to %lld keys are more than one call takes", units, keys);
+    const int splits = pieces_out ? pieces_out : paged_tiles_pieces(ctx, a);
+    size_t bytes = 0;
+    if (!pieces_out && splits > 1) {
+        const size_t po = ((size_t)splits * a.hkv * rows * DP * 4 + 255) & ~(size_t)255;
+        a.po = reinterpret_cast<float *>(ws), a.pml = reinterpret_cast<float2 *>(ws + po);
+        bytes = po + (size_t)splits * a.hkv * rows * 8;
+        a.pieces = splits;
+    }
+    *need = bytes;
+    if (!a.q)
+        return PETB200_OK;
+    if (bytes > ws_bytes)
+        return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes, %zu are needed", ws_bytes, bytes);
+    if (units == 0)
+        return PETB200_OK;
+    if (int rc = raise_smem(ctx, (const void *)k_paged_tiles<T, DP>, C::SMEM))
+        return rc;
+    launch_pdl(k_paged_tiles<T, DP>, dim3((unsigned)(units * splits)), kTileThreads, C::SMEM, s, a, splits, (int)(pieces_out || splits > 1));
+    int rc = launched(ctx, "k_paged_tiles");
+    if (rc || pieces_out || splits == 1)
+        return rc;
+    launch_pdl(k_paged_join_rows<T, DP>, dim3((unsigned)((rows * a.hkv + 3) / 4)), 128, 0, s, a);
+    return launched(ctx, "k_paged_join_rows");
+}
+
+} // namespace
+
+int paged_tiles_pieces(petb200_ctx *ctx, const PagedArgs &a) {
+    const bool one = a.s.kv_lens == nullptr;
+    const long long rows = (long long)a.s.tokens * a.group, seqs = one ? 1 : a.s.seqs;
+    const long long units = std::max(1ll, (rows / (2 * kTileRows) + seqs) * a.hkv);
+    const long long keys = (long long)a.s.n0 + (one ? 0 : (long long)a.s.width * a.s.page_size);
+    // Keys are split until every SM has a block, but no finer than four tiles of them: a piece costs its rows' sums through memory twice.
+    return (int)std::max(1ll, std::min({(long long)ctx->sm_count / units, keys / (4 * kTileKeys), 32ll}));
+}
+
+int paged_tiles_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
+    const bool wide = a.dim > 64;
+    if (dtype == PETB200_F16)
+        return wide ? tiles_launch<__half, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s) : tiles_launch<__half, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+    return wide ? tiles_launch<__nv_bfloat16, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s)
+                : tiles_launch<__nv_bfloat16, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+}
+
+} // namespace petb200

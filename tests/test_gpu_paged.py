@@ -165,6 +165,54 @@ def test_large_scores_and_a_scale(ctx, dtype):
     c.check(c.attend(ctx, scale=0.5), scale=0.5)
 
 
+# Rows around a tile of 128 and a pair of tiles, keys around a tile of 128, heads narrower than the tile's 64 or 128 columns
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [8, 64, 72, 128])
+@pytest.mark.parametrize("rows,keys", [(64, 64), (127, 127), (128, 128), (129, 129), (255, 400), (256, 256), (257, 513)])
+def test_tiles_of_rows_and_keys(ctx, dtype, dim, rows, keys):
+    c = Case(dtype, [rows], [keys], 1, 1, dim, 16, device="cuda")
+    c.check(c.attend(ctx))
+    ctx.sync_check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,lens,heads,group", [([100], [6100], 1, 1), ([40, 30], [3000, 31], 2, 5), ([64, 1, 200], [2000, 2500, 200], 1, 2)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_few_rows_on_many_keys_are_split(ctx, dtype, new, lens, heads, group, causal):
+    for layout, page in (("heads", 64), ("gaps", 9)):
+        c = Case(dtype, new, lens, heads, group, 64, page, layout=layout, device="cuda", behind=4)
+        out = torch.full_like(c.q, 5.0).cuda()
+        c.check(c.attend(ctx, causal=causal, out=out), causal=causal)
+        assert (out[c.starts[-1]:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_maximum_that_grows_late(ctx, dtype):
+    """Scores that rise along the keys by far more than the sums' range allows without scaling, and rows that stay at one level."""
+    c = Case(dtype, [130], [900], 1, 1, 64, device="cuda")
+    for j in range(900):
+        page, slot = c.table[0, j // c.page].long(), j % c.page
+        c.k[page, slot] = (torch.randn(1, 64) * 0.1 + j / 100).to(dtype)
+    c.q[:60] = c.q[:60].abs()
+    c.q[60:90] = 0
+    c.check(c.attend(ctx))
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_masked_values_in_split_tiles(ctx, bad):
+    """Non-finite values of v among the newest keys, where the keys are split over blocks: only the rows that see them have them."""
+    c = Case(BF16, [100], [3000], 1, 1, 64, device="cuda")
+    want, tol = c.want()
+    for at, d in ((2950, 5), (2999, 9), (2925, 63)):
+        c.v[c.table[0, at // c.page].long(), at % c.page, 0, d] = bad
+    got = c.attend(ctx).double().cpu()
+    seen = {5: 50, 9: 99, 63: 25}
+    for d in range(64):
+        clean = seen.get(d, 100)
+        assert ((got[:clean, 0, d] - want[:clean, 0, d]).abs() <= tol[:clean, 0, d]).all()
+        assert not torch.isfinite(got[clean:, 0, d]).any()
+
+
 def test_strided_queries_and_output(ctx):
     c = Case(BF16, [3, 70], [90, 70], 2, 3, 64, device="cuda")
     wide = torch.randn(c.tokens, 10, 64, device="cuda").to(BF16)
