@@ -39,13 +39,18 @@ struct PagedSeqs {
         return min(max(n, 0), most);
     }
     __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
-    // The page that holds key `key` of sequence b (keys [0, n0) are the shared ones), its place in `slot`; -1: not a page.
-    __device__ __forceinline__ int page(int b, int key, int &slot) const {
+    // The table's entry for key `key` of sequence b (keys [0, n0) are the shared ones), the key's place in that page in `slot`.
+    __device__ __forceinline__ int entry(int b, int key, int &slot) const {
         const int own_key = key - n0;
         const int k = own_key < 0 ? key : own_key, i = page_of(k);
         slot = k - i * page_size;
-        const int p = own_key < 0 ? __ldg(table0 + i) : __ldg(table + b * tstride + i);
-        if ((unsigned)p < (unsigned)pages)
+        return own_key < 0 ? __ldg(table0 + i) : __ldg(table + b * tstride + i);
+    }
+    __device__ __forceinline__ bool is_page(int p) const { return (unsigned)p < (unsigned)pages; }
+    // The page, or -1 (reported) where the entry is none.
+    __device__ __forceinline__ int page(int b, int key, int &slot) const {
+        const int p = entry(b, key, slot);
+        if (is_page(p))
             return p;
         atomicOr(status, kStatusPage);
         return -1;

@@ -36,10 +36,10 @@ template <int DP> struct TileCfg {
     static constexpr int STAGE = kTileKeys * DP * 2;
     static constexpr int NS = DP == 128 ? 5 : 8; // stages of the ring, K and V in turn
     static constexpr int Q = 2 * kTileRows * DP * 2;
-    static constexpr int SMEM = 1024 + Q + NS * STAGE;
+    static constexpr int SMEM = Q + NS * STAGE + 2048 + 512; // tiles (at the block's base, which is 1024-byte aligned), row table, control
     static constexpr int CPR = DP / 8, RP = 128 / CPR, NP = 128 / RP; // pieces of a row; rows of a pass of the 128 threads; passes
 };
-static_assert(TileCfg<128>::SMEM <= 227 * 1024 - 512, "shared memory of a block");
+static_assert(TileCfg<128>::SMEM <= 227 * 1024, "shared memory of a block");
 
 struct TileCtl {
     uint64_t q_full, full[8], empty[8], s_full[2], p_full[2], o_full[2];
@@ -47,6 +47,15 @@ struct TileCtl {
     int abort, bad; // bad: non-finite values of V were taken out
     int b, unit;
 };
+static_assert(sizeof(TileCtl) <= 512, "control block");
+
+// Barrier among `threads` threads that answers whether `v` held for all of them.
+__device__ __forceinline__ bool named_bar_all(int id, int threads, bool v) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %3, 0;\n\tbar.red.and.pred p, %1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(r) : "r"(id), "r"(threads), "r"((uint32_t)v) : "memory");
+    return r != 0;
+}
 
 // D[tmem] (+)= A[smem] * B[smem], 16-bit inputs, fp32 accumulate; one thread issues.
 __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -86,12 +95,17 @@ template <typename T> __device__ __forceinline__ uint32_t word_clean(uint32_t w)
 
 template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1) k_paged_tiles(const PagedArgs a, int splits, int to_pieces) {
     using C = TileCfg<DP>;
-    extern __shared__ unsigned char smem_raw[];
-    __shared__ TileCtl ctl;
-    unsigned char *smem = smem_raw + ((1024 - (ptx::smem_u32(smem_raw) & 1023)) & 1023);
+    extern __shared__ __align__(1024) unsigned char smem[];
+    int2 *row_table = reinterpret_cast<int2 *>(smem + C::Q + C::NS * C::STAGE); // [2][128]: a tile's keys as {page (-1: zeros), slot}
+    TileCtl &ctl = *reinterpret_cast<TileCtl *>(smem + C::Q + C::NS * C::STAGE + 2048);
     const uint32_t q_s = ptx::smem_u32(smem), ring = q_s + C::Q;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     volatile int *abort_flag = &ctl.abort;
+    if (q_s & 1023) { // (the swizzle counts from 1024-byte boundaries; a block's dynamic memory begins on one)
+        if (threadIdx.x == 0)
+            atomicOr(a.s.status, 1);
+        return;
+    }
 
     if (threadIdx.x == 0) {
         ptx::mbar_init(&ctl.q_full, 128);
@@ -205,15 +219,26 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                 ptx::mbar_arrive(told == 0 ? &ctl.q_full : &ctl.full[(told - 1) % C::NS]);
                 ++told;
             };
+            // A thread looks up one key of the tile, a tile ahead, and leaves it in the row table; the copies read the places there.
+            int page = 0, slot = 0;
+            auto look = [&](int j) {
+                if (j * kTileKeys + lt < n)
+                    page = a.s.entry(b, j * kTileKeys + lt, slot);
+            };
             bool ok = true;
-            for (int j = k0; j < k1 && ok; ++j) {
-                int pid[C::NP];
-#pragma unroll
-                for (int i = 0; i < C::NP; ++i) {
-                    const int key = j * kTileKeys + i * C::RP + r0;
-                    int slot;
-                    pid[i] = key < n ? a.s.page(b, key, slot) : -1;
-                }
+            if (steps > 0)
+                look(k0);
+            for (int j = k0; j < k1; ++j) {
+                int2 *rows_j = row_table + (j & 1) * kTileKeys;
+                const bool in = j * kTileKeys + lt < n, is_page = a.s.is_page(page);
+                if (in && !is_page)
+                    atomicOr(a.s.status, kStatusPage);
+                rows_j[lt] = make_int2(in && is_page ? page : -1, slot);
+                if (j + 1 < k1)
+                    look(j + 1);
+                ok = named_bar_all(1, 128, ok); // (all of them leave together)
+                if (!ok)
+                    break;
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
                     const int item = issued - 1, s = item % C::NS, use = item / C::NS;
@@ -229,10 +254,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                         const long long sp = v ? a.vp : a.kp, ss = v ? a.vs : a.ks;
 #pragma unroll
                         for (int i = 0; i < C::NP; ++i) {
-                            const int key = j * kTileKeys + i * C::RP + r0, own_key = key < a.s.n0 ? key : key - a.s.n0;
-                            const int slot = own_key - a.s.page_of(own_key) * a.s.page_size;
-                            const bool in = col && pid[i] >= 0;
-                            cp_async_16_or_zero(dst + i * (C::RP * 128), in ? base + (long long)pid[i] * sp + (long long)slot * ss : base, in ? 16 : 0);
+                            const int2 at = rows_j[i * C::RP + r0];
+                            const bool in = col && at.x >= 0;
+                            cp_async_16_or_zero(dst + i * (C::RP * 128), base + (in ? (long long)at.x * sp + (long long)at.y * ss : 0), in ? 16 : 0);
                         }
                         asm volatile("cp.async.commit_group;" ::: "memory");
                         ++issued;
@@ -343,36 +367,30 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                         m = to;
                         l *= f;
 #pragma unroll
-                        for (int c = 0; c < DP / 32; ++c) {
-                            uint32_t o[32];
-                            ptx::tmem_ld_32x32(o_t + c * 32, o);
+                        for (int c = 0; c < DP / 16; ++c) {
+                            uint32_t o[16];
+                            ptx::tmem_ld_32x16(o_t + c * 16, o);
                             ptx::tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i)
+                            for (int i = 0; i < 16; ++i)
                                 o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            ptx::tmem_st_32x32(o_t + c * 32, o);
+                            ptx::tmem_st_32x16(o_t + c * 16, o);
                         }
                     }
                     const float z = m == -INFINITY ? 0.f : -m;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
+                        uint32_t p[16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float p = exp2_approx(fmaf(__uint_as_float(s[c][i]), a.sl2, z));
-                            sum[i & 3] += p;
-                            s[c][i] = __float_as_uint(p);
+                        for (int i = 0; i < 16; ++i) {
+                            const float x = exp2_approx(fmaf(__uint_as_float(s[c][2 * i]), a.sl2, z)), y = exp2_approx(fmaf(__uint_as_float(s[c][2 * i + 1]), a.sl2, z));
+                            sum[i & 1] += x, sum[2 + (i & 1)] += y;
+                            p[i] = pack2<T>(x, y);
                         }
+                        ptx::tmem_st_32x16(s_t + c * 16, p);
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t p[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            p[i] = pack2<T>(__uint_as_float(s[2 * c + (i >> 4)][2 * (i & 15)]), __uint_as_float(s[2 * c + (i >> 4)][2 * (i & 15) + 1]));
-                        ptx::tmem_st_32x32(s_t + c * 32, p);
-                    }
                     ptx::tmem_st_wait();
                     ptx::tc_fence_before();
                     ptx::mbar_arrive(&ctl.p_full[t]);
@@ -529,7 +547,7 @@ int tiles_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_
 int paged_tiles_pieces(petb200_ctx *ctx, const PagedArgs &a) {
     const bool one = a.s.kv_lens == nullptr;
     const long long rows = (long long)a.s.tokens * a.group, seqs = one ? 1 : a.s.seqs;
-    const long long units = std::max(1ll, (rows / (2 * kTileRows) + seqs) * a.hkv);
+    const long long units = std::max(seqs, (rows + kTileRows) / (2 * kTileRows)) * a.hkv; // about: uneven sequences make a few more
     const long long keys = (long long)a.s.n0 + (one ? 0 : (long long)a.s.width * a.s.page_size);
     // Keys are split until every SM has a block, but no finer than four tiles of them: a piece costs its rows' sums through memory twice.
     return (int)std::max(1ll, std::min({(long long)ctx->sm_count / units, keys / (4 * kTileKeys), 32ll}));
