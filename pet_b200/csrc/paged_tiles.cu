@@ -252,11 +252,20 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                         const uint32_t dst = ring + s * C::STAGE + at0;
                         const T *base = v ? vc : kc;
                         const long long sp = v ? a.vp : a.kp, ss = v ? a.vs : a.ks;
+                        // (places of eight rows are read before their copies: a copy's asm keeps later reads behind it)
 #pragma unroll
-                        for (int i = 0; i < C::NP; ++i) {
-                            const int2 at = rows_j[i * C::RP + r0];
-                            const bool in = col && at.x >= 0;
-                            cp_async_16_or_zero(dst + i * (C::RP * 128), base + (in ? (long long)at.x * sp + (long long)at.y * ss : 0), in ? 16 : 0);
+                        for (int i0 = 0; i0 < C::NP; i0 += 8) {
+                            const T *src[8];
+                            int bytes[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int2 at = rows_j[(i0 + i) * C::RP + r0];
+                                bytes[i] = col && at.x >= 0 ? 16 : 0;
+                                src[i] = base + (bytes[i] ? (long long)at.x * sp + (long long)at.y * ss : 0);
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                cp_async_16_or_zero(dst + (i0 + i) * (C::RP * 128), src[i], bytes[i]);
                         }
                         asm volatile("cp.async.commit_group;" ::: "memory");
                         ++issued;
