@@ -171,9 +171,21 @@ struct DeviceGuard {
     }
 };
 
-int check_cache(petb200_ctx *ctx, const char *what, const petb200_kv_cache *c, const petb200_kv_seqs *s) {
-    if (!c || !s)
+// The stride of an extent of one is never used, and may be anything.
+petb200_kv_cache plain_strides(petb200_kv_cache c) {
+    if (c.pages <= 1)
+        c.k_page = c.v_page = 0;
+    if (c.page_size == 1)
+        c.k_slot = c.v_slot = 0;
+    if (c.heads == 1)
+        c.k_head = c.v_head = 0;
+    return c;
+}
+
+int check_cache(petb200_ctx *ctx, const char *what, const petb200_kv_cache *cache, const petb200_kv_seqs *s) {
+    if (!cache || !s)
         return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
+    const petb200_kv_cache plain = plain_strides(*cache), *c = &plain;
     if (c->dtype < PETB200_F32 || c->dtype > PETB200_BF16)
         return fail(ctx, PETB200_ERR_INVALID, "%s: unknown type %d", what, c->dtype);
     if (c->pages < 0 || c->page_size <= 0 || c->heads <= 0 || c->dim <= 0 || s->seqs < 0 || s->tokens < 0 || s->table_width < 0)
@@ -211,8 +223,9 @@ PagedSeqs device_seqs(petb200_ctx *ctx, const petb200_kv_cache *c, const petb200
     return d;
 }
 
-PagedArgs attention_args(petb200_ctx *ctx, const petb200_kv_cache *c, const petb200_kv_seqs *s, int q_heads) {
+PagedArgs attention_args(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *s, int q_heads) {
     PagedArgs a;
+    const petb200_kv_cache plain = plain_strides(*cache), *c = &plain;
     a.s = device_seqs(ctx, c, s);
     a.kc = c->k, a.vc = c->v;
     a.kp = c->k_page, a.ks = c->k_slot, a.kh = c->k_head, a.vp = c->v_page, a.vs = c->v_slot, a.vh = c->v_head;
@@ -332,8 +345,9 @@ extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *c
             a.vec = 0;
     }
     a.y[0] = q_out.p, a.y_tok = q_out.tok, a.y_head[0] = q_out.head;
-    a.y[1] = cache->k, a.y_page[1] = cache->k_page, a.y_slot[1] = cache->k_slot, a.y_head[1] = cache->k_head;
-    a.y[2] = cache->v, a.y_page[2] = cache->v_page, a.y_slot[2] = cache->v_slot, a.y_head[2] = cache->v_head;
+    const petb200_kv_cache c = plain_strides(*cache);
+    a.y[1] = c.k, a.y_page[1] = c.k_page, a.y_slot[1] = c.k_slot, a.y_head[1] = c.k_head;
+    a.y[2] = c.v, a.y_page[2] = c.v_page, a.y_slot[2] = c.v_slot, a.y_head[2] = c.v_head;
     a.dim = cache->dim, a.rot = rotary, a.interleaved = interleaved != 0, a.pos0 = pos0, a.inv_freq = inv_freq;
     if ((long long)(a.heads[0] + a.heads[1] + a.heads[2]) * a.dim > 1 << 24)
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: a token of more than 2^24 values", what);

@@ -12,12 +12,15 @@
 // The maximum moves only where a row's grows by more than 2^8 over the one in use (then O and l are scaled, by the softmax warps): the
 // sums stay within range and any m gives the same quotient.
 //
-// K and V rows come by 16-byte asynchronous copies in the 128-byte swizzle (piece c of row r at c ^ (r & 7)): the pages may have any size and
-// strides, and keys past the end arrive as zeros whatever the page holds there.  V is the second product's B operand as it
-// lies, its rows along K ("MN-major").  Per 128 keys and SM that is 64 KB, 4096 copies by four warps, an eighth of the issue slots.
+// K and V tiles are fetched by TMA, a box per page (or part of a page) and 64 columns, in the 128-byte swizzle (16-byte piece c of row r at
+// c ^ (r & 7)); V is the second product's B operand as it lies, its rows along K ("MN-major").  Pages that do not fit the tiles (a
+// page size that neither divides 128 nor is a multiple of it, or is below 8) come by 16-byte asynchronous copies of four warps
+// instead, which is issue-bound: 5.1 k cycles per 128 keys.  Keys count in tiles from the first shared key and again from the first own
+// key, so that a tile never straddles the two.
 //
-// A masked key's score is replaced before the maximum.  Where some row of the unit does not see some key of a tile, the fetching warps
-// look for non-finite values of V and take them out (0 x infinity would be NaN); the rows that do see them get them back at the end.
+// A masked key's score is replaced before the maximum.  Rows of V that no row of the unit sees are zeros in shared memory, whatever
+// the page holds there.  Where some row of the unit does not see some key of a tile, the fetching warps look for non-finite values of
+// V and take them out (0 x infinity would be NaN); the rows that do see them get them back at the end.
 #include "paged.cuh"
 #include "tc_ptx.cuh"
 #include <algorithm>
@@ -37,12 +40,13 @@ template <int DP> struct TileCfg {
     static constexpr int NS = DP == 128 ? 5 : 8; // stages of the ring, K and V in turn
     static constexpr int Q = 2 * kTileRows * DP * 2;
     static constexpr int SMEM = Q + NS * STAGE + 2048 + 512; // tiles (at the block's base, which is 1024-byte aligned), row table, control
+    static constexpr int SUBS = DP / 64;         // blocks of 64 columns (128 bytes) of a tile
     static constexpr int CPR = DP / 8, RP = 128 / CPR, NP = 128 / RP; // pieces of a row; rows of a pass of the 128 threads; passes
 };
 static_assert(TileCfg<128>::SMEM <= 227 * 1024, "shared memory of a block");
 
 struct TileCtl {
-    uint64_t q_full, full[8], empty[8], s_full[2], p_full[2], o_full[2];
+    uint64_t q_full, raw, full[8], empty[8], s_full[2], p_full[2], o_full[2]; // raw: a V tile that is looked over before it is full
     uint32_t tmem;
     int abort, bad; // bad: non-finite values of V were taken out
     int b, unit;
@@ -93,7 +97,8 @@ template <typename T> __device__ __forceinline__ uint32_t word_clean(uint32_t w)
     return ((w & e) == e ? 0u : w & 0xffffu) | (((w >> 16) & e) == e ? 0u : w & 0xffff0000u);
 }
 
-template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1) k_paged_tiles(const PagedArgs a, int splits, int to_pieces) {
+template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
+    k_paged_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedArgs a, int splits, int to_pieces, int tma) {
     using C = TileCfg<DP>;
     extern __shared__ __align__(1024) unsigned char smem[];
     int2 *row_table = reinterpret_cast<int2 *>(smem + C::Q + C::NS * C::STAGE); // [2][128]: a tile's keys as {page (-1: zeros), slot}
@@ -109,8 +114,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
 
     if (threadIdx.x == 0) {
         ptx::mbar_init(&ctl.q_full, 128);
+        ptx::mbar_init(&ctl.raw, 1);
         for (int i = 0; i < C::NS; ++i) {
-            ptx::mbar_init(&ctl.full[i], 128);
+            ptx::mbar_init(&ctl.full[i], tma ? 1 : 128);
             ptx::mbar_init(&ctl.empty[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
@@ -177,10 +183,15 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
         int t0;
         const int ql = tokens_of(b, t0), own = one ? 0 : a.s.own(b), rows = min(2 * kTileRows, ql * a.group - row0);
         const int tiles = rows > kTileRows ? 2 : 1;
-        const int n = a.s.visible((row0 + rows - 1) / a.group, ql, own, a.causal);  // keys that the last row sees
-        const int full = a.s.visible(row0 / a.group, ql, own, a.causal);            // keys that every row sees
-        const int all = (n + kTileKeys - 1) / kTileKeys;
+        // own keys that the last row sees, and the first; the rows see all shared keys
+        const int n0 = a.s.n0, own_last = a.s.visible((row0 + rows - 1) / a.group, ql, own, a.causal) - n0;
+        const int own_first = a.s.visible(row0 / a.group, ql, own, a.causal) - n0;
+        const int tiles0 = (n0 + kTileKeys - 1) / kTileKeys, all = tiles0 + (own_last + kTileKeys - 1) / kTileKeys;
         const int k0 = (int)((long long)all * split / splits), k1 = (int)((long long)all * (split + 1) / splits), steps = k1 - k0;
+        // A tile's first key (counted in its part), its part's end, and the key of the whole sequence that its first is
+        auto first_key = [&](int j) { return (j < tiles0 ? j : j - tiles0) * kTileKeys; };
+        auto part_end = [&](int j) { return j < tiles0 ? n0 : own_last; };
+        auto whole_key = [&](int j) { return first_key(j) + (j < tiles0 ? 0 : n0); };
 
         if (warp >= 8 && warp < 12) {
             ptx::reg_dealloc<kOtherRegs>();
@@ -198,87 +209,158 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             }
-            int issued = steps > 0 ? 1 : 0, told = 0; // of Q, K 0, V 0, K 1, ...
-            auto tell = [&]() {                      // the oldest of them has arrived: its own copies, then everyone's
-                if (told > 0 && !(told & 1)) {
-                    const int j = k0 + told / 2 - 1, s = (told - 1) % C::NS;
-                    if ((j + 1) * kTileKeys > full) {
-                        unsigned char *p = smem + C::Q + s * C::STAGE + at0;
-#pragma unroll 1
-                        for (int i = 0; i < C::NP; ++i) {
-                            uint4 *w = reinterpret_cast<uint4 *>(p + i * (C::RP * 128));
-                            const uint4 x = *w;
-                            if (word_bad<T>(x.x) || word_bad<T>(x.y) || word_bad<T>(x.z) || word_bad<T>(x.w)) {
-                                *w = make_uint4(word_clean<T>(x.x), word_clean<T>(x.y), word_clean<T>(x.z), word_clean<T>(x.w));
-                                *(volatile int *)&ctl.bad = 1;
-                            }
-                        }
+            // Looks over this thread's pieces of the V tile in stage `st`: rows past the part's end become zeros, non-finite values too
+            // where some row does not see some key of the tile (among shared keys every row sees all).
+            auto scrub = [&](int j, int st) {
+                unsigned char *p = smem + C::Q + st * C::STAGE + at0;
+                const int left = part_end(j) - first_key(j);
+#pragma unroll 4
+                for (int i = 0; i < C::NP; ++i) {
+                    uint4 *w = reinterpret_cast<uint4 *>(p + i * (C::RP * 128));
+                    const uint4 x = *w;
+                    if (i * C::RP + r0 >= left)
+                        *w = make_uint4(0u, 0u, 0u, 0u);
+                    else if (j >= tiles0 && (word_bad<T>(x.x) || word_bad<T>(x.y) || word_bad<T>(x.z) || word_bad<T>(x.w))) {
+                        *w = make_uint4(word_clean<T>(x.x), word_clean<T>(x.y), word_clean<T>(x.z), word_clean<T>(x.w));
+                        *(volatile int *)&ctl.bad = 1;
                     }
                 }
+            };
+            auto partly = [&](int j) { return first_key(j) + kTileKeys > (j < tiles0 ? n0 : own_first); };
+            if (tma) {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
                 ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive(told == 0 ? &ctl.q_full : &ctl.full[(told - 1) % C::NS]);
-                ++told;
-            };
-            // A thread looks up one key of the tile, a tile ahead, and leaves it in the row table; the copies read the places there.
-            int page = 0, slot = 0;
-            auto look = [&](int j) {
-                if (j * kTileKeys + lt < n)
-                    page = a.s.entry(b, j * kTileKeys + lt, slot);
-            };
-            bool ok = true;
-            if (steps > 0)
-                look(k0);
-            for (int j = k0; j < k1; ++j) {
-                int2 *rows_j = row_table + (j & 1) * kTileKeys;
-                const bool in = j * kTileKeys + lt < n, is_page = a.s.is_page(page);
-                if (in && !is_page)
-                    atomicOr(a.s.status, kStatusPage);
-                rows_j[lt] = make_int2(in && is_page ? page : -1, slot);
-                if (j + 1 < k1)
-                    look(j + 1);
-                ok = named_bar_all(1, 128, ok); // (all of them leave together)
-                if (!ok)
-                    break;
-#pragma unroll
-                for (int v = 0; v < 2; ++v) {
-                    const int item = issued - 1, s = item % C::NS, use = item / C::NS;
-                    if (use > 0 && !ptx::mbar_try_wait(&ctl.empty[s], (use - 1) & 1)) {
-                        asm volatile("cp.async.wait_group 0;" ::: "memory"); // whoever empties the stage may be waiting for these
-                        while (told < issued)
-                            tell();
-                        ok = ok && ptx::mbar_wait(&ctl.empty[s], (use - 1) & 1, abort_flag);
-                    }
-                    if (ok) {
-                        const uint32_t dst = ring + s * C::STAGE + at0;
-                        const T *base = v ? vc : kc;
-                        const long long sp = v ? a.vp : a.kp, ss = v ? a.vs : a.ks;
-                        // (places of eight rows are read before their copies: a copy's asm keeps later reads behind it)
-#pragma unroll
-                        for (int i0 = 0; i0 < C::NP; i0 += 8) {
-                            const T *src[8];
-                            int bytes[8];
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) {
-                                const int2 at = rows_j[(i0 + i) * C::RP + r0];
-                                bytes[i] = col && at.x >= 0 ? 16 : 0;
-                                src[i] = base + (bytes[i] ? (long long)at.x * sp + (long long)at.y * ss : 0);
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                cp_async_16_or_zero(dst + (i0 + i) * (C::RP * 128), src[i], bytes[i]);
+                if (steps > 0)
+                    ptx::mbar_arrive(&ctl.q_full);
+                const int box = min(a.s.page_size, kTileKeys), boxes = kTileKeys / box, sub = lane % C::SUBS, mine = lane / C::SUBS;
+                // A lane looks up the page of its box, a tile ahead.  No page (past the keys, or not one): a page past the last, zeros.
+                int page = 0, slot = 0;
+                auto look = [&](int j) {
+                    const int key = first_key(j) + mine * box;
+                    page = a.s.pages;
+                    if (mine < boxes && key < part_end(j)) {
+                        page = a.s.entry(b, whole_key(j) + mine * box, slot);
+                        if (!a.s.is_page(page)) {
+                            atomicOr(a.s.status, kStatusPage);
+                            page = a.s.pages;
                         }
-                        asm volatile("cp.async.commit_group;" ::: "memory");
-                        ++issued;
-                        if (issued - told > kLag) {
-                            asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-                            tell();
+                    }
+                };
+                if (warp == 8 && steps > 0)
+                    look(k0);
+                bool ok = true;
+                int looked = 0; // V tiles looked over so far
+                for (int j = k0; j < k1; ++j) {
+                    const bool over = partly(j);
+                    const int iv = 2 * (j - k0) + 1, sv = iv % C::NS;
+                    if (warp == 8) {
+                        const int p = page, sl = slot;
+                        if (j + 1 < k1)
+                            look(j + 1);
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) {
+                            const int item = 2 * (j - k0) + v, st = item % C::NS, use = item / C::NS;
+                            if (use > 0)
+                                ok = ok && ptx::mbar_wait_warp(&ctl.empty[st], (use - 1) & 1, abort_flag);
+                            if (ok) {
+                                uint64_t *bar = v && over ? &ctl.raw : &ctl.full[st];
+                                if (lane == 0)
+                                    ptx::mbar_expect_tx(bar, C::STAGE);
+                                __syncwarp();
+                                if (mine < boxes)
+                                    ptx::tma_load_4d(smem + C::Q + st * C::STAGE + sub * (kTileKeys * 128) + mine * box * 128, v ? &vmap : &kmap, bar, sub * 64, sl, h, p);
+                            }
+                        }
+                    } else if (!over)
+                        continue;
+                    if (over) { // (warps 9 to 11 come here for these tiles alone, in step with warp 8)
+                        ok = named_bar_all(1, 128, ok);
+                        if (!ok)
+                            break;
+                        ok = ptx::mbar_wait(&ctl.raw, looked++ & 1, abort_flag);
+                        if (ok)
+                            scrub(j, sv);
+                        ptx::fence_proxy_async_smem();
+                        ok = named_bar_all(1, 128, ok);
+                        if (!ok)
+                            break;
+                        if (lt == 0)
+                            ptx::mbar_arrive(&ctl.full[sv]);
+                    }
+                }
+            } else {
+                int issued = steps > 0 ? 1 : 0, told = 0; // of Q, K 0, V 0, K 1, ...
+                auto tell = [&]() {                      // the oldest of them has arrived: its own copies, then everyone's
+                    if (told > 0 && !(told & 1)) {
+                        const int j = k0 + told / 2 - 1;
+                        if (partly(j))
+                            scrub(j, (told - 1) % C::NS);
+                    }
+                    ptx::fence_proxy_async_smem();
+                    ptx::mbar_arrive(told == 0 ? &ctl.q_full : &ctl.full[(told - 1) % C::NS]);
+                    ++told;
+                };
+                // A thread looks up one key of the tile, a tile ahead, and leaves it in the row table; the copies read the places there.
+                int page = 0, slot = 0;
+                auto look = [&](int j) {
+                    if (first_key(j) + lt < part_end(j))
+                        page = a.s.entry(b, whole_key(j) + lt, slot);
+                };
+                bool ok = true;
+                if (steps > 0)
+                    look(k0);
+                for (int j = k0; j < k1; ++j) {
+                    int2 *rows_j = row_table + (j & 1) * kTileKeys;
+                    const bool in = first_key(j) + lt < part_end(j), is_page = a.s.is_page(page);
+                    if (in && !is_page)
+                        atomicOr(a.s.status, kStatusPage);
+                    rows_j[lt] = make_int2(in && is_page ? page : -1, slot);
+                    if (j + 1 < k1)
+                        look(j + 1);
+                    ok = named_bar_all(1, 128, ok); // (all of them leave together)
+                    if (!ok)
+                        break;
+#pragma unroll
+                    for (int v = 0; v < 2; ++v) {
+                        const int item = issued - 1, s = item % C::NS, use = item / C::NS;
+                        if (use > 0 && !ptx::mbar_try_wait(&ctl.empty[s], (use - 1) & 1)) {
+                            asm volatile("cp.async.wait_group 0;" ::: "memory"); // whoever empties the stage may be waiting for these
+                            while (told < issued)
+                                tell();
+                            ok = ok && ptx::mbar_wait(&ctl.empty[s], (use - 1) & 1, abort_flag);
+                        }
+                        if (ok) {
+                            const uint32_t dst = ring + s * C::STAGE + at0;
+                            const T *base = v ? vc : kc;
+                            const long long sp = v ? a.vp : a.kp, ss = v ? a.vs : a.ks;
+                            // (places of eight rows are read before their copies: a copy's asm keeps later reads behind it)
+#pragma unroll
+                            for (int i0 = 0; i0 < C::NP; i0 += 8) {
+                                const T *src[8];
+                                int bytes[8];
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) {
+                                    const int2 at = rows_j[(i0 + i) * C::RP + r0];
+                                    bytes[i] = col && at.x >= 0 ? 16 : 0;
+                                    src[i] = base + (bytes[i] ? (long long)at.x * sp + (long long)at.y * ss : 0);
+                                }
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    cp_async_16_or_zero(dst + (i0 + i) * (C::RP * 128), src[i], bytes[i]);
+                            }
+                            asm volatile("cp.async.commit_group;" ::: "memory");
+                            ++issued;
+                            if (issued - told > kLag) {
+                                asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                                tell();
+                            }
                         }
                     }
                 }
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                while (told < issued)
+                    tell();
             }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            while (told < issued)
-                tell();
         } else if (warp >= 12) {
             ptx::reg_dealloc<kOtherRegs>();
             // ---- products ------------------------------------------------------------------------------------------------
@@ -335,7 +417,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
             const int t = warp >> 2, r = t * kTileRows + (warp & 3) * 32 + lane, tok = (row0 + r) / a.group, hd = row0 + r - tok * a.group;
             if (t < tiles) {
                 const bool live = r < rows;
-                const int lim = live ? a.s.visible(tok, ql, own, a.causal) : n; // (rows past the end: zeros of q, nothing is written)
+                const int lim = live ? a.s.visible(tok, ql, own, a.causal) - n0 : own_last; // of its own keys (rows past the end: zeros of q, nothing is written)
                 const int warp_lim = __reduce_min_sync(0xffffffffu, lim);
                 const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
                 float m = -INFINITY, l = 0.f; // m: the maximum in use, times scale log2(e)
@@ -350,9 +432,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                     for (int c = 0; c < 4; ++c)
                         ptx::tmem_ld_32x32(s_t + c * 32, s[c]);
                     ptx::tmem_ld_wait();
-                    const int key0 = (k0 + j) * kTileKeys;
-                    if (key0 + kTileKeys > warp_lim) {
-                        const int see = lim - key0;
+                    const int jj = k0 + j, key0 = first_key(jj);
+                    if (key0 + kTileKeys > (jj < tiles0 ? n0 : warp_lim)) {
+                        const int see = (jj < tiles0 ? n0 : lim) - key0;
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -364,15 +446,18 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                     for (int c = 0; c < 4; ++c) {
                         mx[c] = __uint_as_float(s[c][0]);
 #pragma unroll
-                        for (int i = 1; i < 32; ++i)
-                            mx[c] = fmaxf(mx[c], __uint_as_float(s[c][i]));
+                        for (int i = 1; i < 31; i += 2)
+                            mx[c] = ptx::max3_nan(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+                        mx[c] = ptx::max3_nan(mx[c], mx[c], __uint_as_float(s[c][31]));
                     }
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.sl2;
+                    float top = ptx::max3_nan(ptx::max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.sl2;
+                    if (!(top < INFINITY))
+                        top = NAN; // the formula's inf - inf, or a score that is none: the row's result is NaN
                     if (j == 0)
                         m = top;
-                    else if (__any_sync(0xffffffffu, top - m > kGrowth)) {
+                    else if (__any_sync(0xffffffffu, top - m > kGrowth || top != top)) {
                         // (the product with the tile before is done: its scores' successor was behind it in the pipe)
-                        const float to = fmaxf(m, top), f = m == to ? 1.f : exp2_approx(m - to);
+                        const float to = top != top || m != m ? NAN : fmaxf(m, top), f = m == to ? 1.f : exp2_approx(m - to);
                         m = to;
                         l *= f;
 #pragma unroll
@@ -387,19 +472,22 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                     }
                     const float z = m == -INFINITY ? 0.f : -m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float2 sl2 = make_float2(a.sl2, a.sl2), zz = make_float2(z, z);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         uint32_t p[16];
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const float x = exp2_approx(fmaf(__uint_as_float(s[c][2 * i]), a.sl2, z)), y = exp2_approx(fmaf(__uint_as_float(s[c][2 * i + 1]), a.sl2, z));
-                            sum[i & 1] += x, sum[2 + (i & 1)] += y;
-                            p[i] = pack2<T>(x, y);
+                            float2 x = ptx::fma_f32x2(make_float2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), sl2, zz);
+                            x.x = exp2_approx(x.x), x.y = exp2_approx(x.y);
+                            sum[i & 1] = ptx::add_f32x2(sum[i & 1], x);
+                            p[i] = pack2<T>(x.x, x.y);
                         }
                         ptx::tmem_st_32x16(s_t + c * 16, p);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    sum[0] = ptx::add_f32x2(sum[0], sum[1]);
+                    l += sum[0].x + sum[0].y;
                     ptx::tmem_st_wait();
                     ptx::tc_fence_before();
                     ptx::mbar_arrive(&ctl.p_full[t]);
@@ -409,8 +497,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                     ok = ptx::mbar_wait_warp(&ctl.o_full[t], 0, abort_flag);
                 if (ok) {
                     ptx::tc_fence_after();
-                    const int key_a = k0 * kTileKeys, key_b = min(lim, k1 * kTileKeys);
-                    const bool seen = key_b > key_a; // this row sees some of this block's keys
+                    const int key_a = max(k0 - tiles0, 0) * kTileKeys, key_b = min(lim, (k1 - tiles0) * kTileKeys); // its own keys here
+                    const bool seen = steps > 0 && (k0 < tiles0 || key_b > key_a); // this row sees some of this block's keys
                     const long long grow = (long long)(t0 + tok) * a.group + hd, at = ((long long)split * a.hkv + h) * ((long long)a.s.tokens * a.group) + grow;
                     const bool bad = steps > 0 && *(volatile int *)&ctl.bad;
                     const float inv = 1.f / l;
@@ -430,9 +518,9 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                                 o[i] = 0u;
                         }
                         if (bad && live) {
-                            for (int key = max(key_a, full / kTileKeys * kTileKeys); key < key_b; ++key) {
+                            for (int key = max(key_a, own_first / kTileKeys * kTileKeys); key < key_b; ++key) {
                                 int slot;
-                                const int p = a.s.page(b, key, slot);
+                                const int p = a.s.page(b, n0 + key, slot);
                                 const T *v = (const T *)a.vc + (long long)p * a.vp + (long long)slot * a.vs + (long long)h * a.vh + c * 32;
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
@@ -516,6 +604,24 @@ template <typename T, int DP> __global__ void __launch_bounds__(128) k_paged_joi
             make_uint2(pack2<T>(v.x * f, v.y * f), pack2<T>(v.z * f, v.w * f));
 }
 
+// The pool as TMA sees it: boxes of up to 128 slots x 64 values of one page and head.  False where the pages do not fit the tiles.
+template <typename T> bool page_map(const PagedArgs &a, const void *pool, long long page, long long slot, long long head, CUtensorMap &map) {
+    const int size = a.s.page_size;
+    EncodeTiledFn enc = encode_fn();
+    if (!enc || size < 8 || a.s.pages < 1 || (size < kTileKeys ? kTileKeys % size : size % kTileKeys))
+        return false;
+    if ((slot == 0 && size > 1) || (head == 0 && a.hkv > 1) || (page == 0 && a.s.pages > 1)) // (an expanded pool)
+        return false;
+    auto bytes = [](long long stride) { return (cuuint64_t)(stride ? stride * 2 : 16); }; // (of an extent of one)
+    const cuuint64_t dims[4] = {(cuuint64_t)a.dim, (cuuint64_t)size, (cuuint64_t)a.hkv, (cuuint64_t)a.s.pages}, strides[3] = {bytes(slot), bytes(head), bytes(page)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(size, kTileKeys), 1, 1}, step[4] = {1, 1, 1, 1};
+    if (strides[0] >> 40 || strides[1] >> 40 || strides[2] >> 40)
+        return false;
+    return enc(&map, std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(pool), dims,
+               strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP>
 int tiles_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
     using C = TileCfg<DP>;
@@ -543,7 +649,9 @@ int tiles_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_
         return PETB200_OK;
     if (int rc = raise_smem(ctx, (const void *)k_paged_tiles<T, DP>, C::SMEM))
         return rc;
-    launch_pdl(k_paged_tiles<T, DP>, dim3((unsigned)(units * splits)), kTileThreads, C::SMEM, s, a, splits, (int)(pieces_out || splits > 1));
+    CUtensorMap kmap{}, vmap{};
+    const int tma = page_map<T>(a, a.kc, a.kp, a.ks, a.kh, kmap) && page_map<T>(a, a.vc, a.vp, a.vs, a.vh, vmap);
+    launch_pdl(k_paged_tiles<T, DP>, dim3((unsigned)(units * splits)), kTileThreads, C::SMEM, s, kmap, vmap, a, splits, (int)(pieces_out || splits > 1), tma);
     int rc = launched(ctx, "k_paged_tiles");
     if (rc || pieces_out || splits == 1)
         return rc;

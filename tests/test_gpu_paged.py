@@ -186,6 +186,28 @@ def test_few_rows_on_many_keys_are_split(ctx, dtype, new, lens, heads, group, ca
         assert (out[c.starts[-1]:] == 5).all()
 
 
+# Pages that are boxes of a tile, hold several tiles, or fit neither; shared keys that end inside a tile and inside a page
+@pytest.mark.parametrize("page", [1, 8, 24, 32, 128, 256, 200])
+@pytest.mark.parametrize("layout", ["slots", "heads", "gaps"])
+@pytest.mark.parametrize("prefix", [0, 75, 700])
+def test_tiles_over_pages_of_any_size(ctx, page, layout, prefix):
+    c = Case(BF16, [70, 0, 140], [70, 9, 560], 2, 2, 128 if page == 32 else 72, page, prefix=prefix, layout=layout, device="cuda")
+    c.check(c.attend(ctx))
+    ctx.sync_check()
+
+
+def test_pools_of_one_page_and_of_one_head_for_all(ctx):
+    """Strides of extents of one are never used; an expanded pool (stride 0) is read as it is."""
+    c = Case(F16, [70], [100], 1, 2, 64, 128, device="cuda")
+    k, v = c.pool(c.k), c.pool(c.v)
+    odd = [t.as_strided(t.shape, (t.stride(0), t.stride(1), 3, 1)) for t in (k, v)]
+    t, n = c.on(c.table), torch.tensor(c.lens, dtype=torch.int32, device="cuda")
+    c.check(ctx.attention_paged(c.on(c.q), *odd, t, n, q_starts=c.on(c.q_starts)))
+    for new in (70, 1):
+        c = Case(F16, [new], [100], 1, 2, 64, 128, device="cuda")
+        c.check(ctx.attention_paged(c.on(c.q), *(c.pool(x).expand(-1, -1, 2, -1) for x in (c.k, c.v)), c.on(c.table), n, q_starts=c.on(c.q_starts)))
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_maximum_that_grows_late(ctx, dtype):
     """Scores that rise along the keys by far more than the sums' range allows without scaling, and rows that stay at one level."""
