@@ -277,7 +277,7 @@ int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, in
 }
 
 int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const int *prefix_table,
-                  int prefix_len, petb200_kv_rows q, petb200_kv_rows out, int q_heads, int causal, float scale, void *workspace,
+                  int prefix_len, const petb200_kv_rows *q, const petb200_kv_rows *out, int q_heads, int causal, float scale, void *workspace,
                   size_t workspace_bytes, cudaStream_t s) {
     if (!ctx)
         return PETB200_ERR_INVALID;
@@ -289,17 +289,17 @@ int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *ca
         return fail(ctx, PETB200_ERR_INVALID, "%s: the scale must be positive, finite and not denormal", what);
     if (seqs->seqs == 0 || seqs->tokens == 0)
         return PETB200_OK;
-    if (!q.p || !out.p || (prefix_len > 0 && !prefix_table))
+    if (!q || !out || !q->p || !out->p || (prefix_len > 0 && !prefix_table))
         return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
     const long long e = 16 / type_size(cache->dtype);
-    if (!on_grid(q.p) || !on_grid(out.p) || q.tok % e || q.head % e || out.tok % e || out.head % e || q.tok < 0 || q.head < 0 || out.tok < 0 || out.head < 0)
+    if (!on_grid(q->p) || !on_grid(out->p) || q->tok % e || q->head % e || out->tok % e || out->head % e || q->tok < 0 || q->head < 0 || out->tok < 0 || out->head < 0)
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
     if (!on_grid(workspace))
         return fail(ctx, PETB200_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
     DeviceGuard guard(ctx->device);
     PagedArgs a = attention_args(ctx, cache, seqs, q_heads);
-    a.q = q.p, a.q_tok = q.tok, a.q_head = q.head;
-    a.out = out.p, a.o_tok = out.tok, a.o_head = out.head;
+    a.q = q->p, a.q_tok = q->tok, a.q_head = q->head;
+    a.out = out->p, a.o_tok = out->tok, a.o_head = out->head;
     a.causal = causal != 0;
     a.sl2 = scale * 1.44269504088896340736f; // log2(e)
     size_t need = 0;
@@ -311,8 +311,8 @@ int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *ca
 
 using namespace petb200;
 
-extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, petb200_kv_rows k,
-                                     petb200_kv_rows v, petb200_kv_rows q, petb200_kv_rows q_out, int q_heads, int src_dtype,
+extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const petb200_kv_rows *k,
+                                     const petb200_kv_rows *v, const petb200_kv_rows *q, const petb200_kv_rows *q_out, int q_heads, int src_dtype,
                                      const float *inv_freq, int rotary, int interleaved, int pos0, petb200_stream stream) {
     const char *what = "kv_append";
     if (!ctx)
@@ -325,26 +325,28 @@ extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *c
         rotary = 0;
     if (rotary < 0 || rotary > cache->dim || rotary % 2)
         return fail(ctx, PETB200_ERR_INVALID, "%s: %d values of %d cannot be turned in pairs", what, rotary, cache->dim);
-    if (q_heads < 0 || (q.p && q_heads == 0))
+    const petb200_kv_rows none{};
+    const petb200_kv_rows src[3] = {q ? *q : none, k ? *k : none, v ? *v : none}, to = q_out ? *q_out : none;
+    const bool with_q = src[0].p != nullptr;
+    if (q_heads < 0 || (with_q && q_heads == 0))
         return fail(ctx, PETB200_ERR_INVALID, "%s: %d query heads", what, q_heads);
     if (seqs->seqs == 0 || seqs->tokens == 0)
         return PETB200_OK;
-    if (!k.p || !v.p || (q.p && !q_out.p))
+    if (!src[1].p || !src[2].p || (with_q && !to.p))
         return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
     const long long e = 16 / type_size(cache->dtype), es = 16 / type_size(src_dtype);
-    if (q.p && (!on_grid(q_out.p) || q_out.tok % e || q_out.head % e || q_out.tok < 0 || q_out.head < 0))
+    if (with_q && (!on_grid(to.p) || to.tok % e || to.head % e || to.tok < 0 || to.head < 0))
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q_out must start on 16-byte boundaries", what);
     AppendArgs a{};
     a.s = device_seqs(ctx, cache, seqs);
-    const petb200_kv_rows src[3] = {q, k, v};
     a.vec = 1;
     for (int i = 0; i < 3; ++i) {
-        a.heads[i] = i ? cache->heads : (q.p ? q_heads : 0);
+        a.heads[i] = i ? cache->heads : (with_q ? q_heads : 0);
         a.x[i] = src[i].p, a.x_tok[i] = src[i].tok, a.x_head[i] = src[i].head;
         if (a.heads[i] && (!on_grid(src[i].p) || src[i].tok % es || src[i].head % es))
             a.vec = 0;
     }
-    a.y[0] = q_out.p, a.y_tok = q_out.tok, a.y_head[0] = q_out.head;
+    a.y[0] = to.p, a.y_tok = to.tok, a.y_head[0] = to.head;
     const petb200_kv_cache c = plain_strides(*cache);
     a.y[1] = c.k, a.y_page[1] = c.k_page, a.y_slot[1] = c.k_slot, a.y_head[1] = c.k_head;
     a.y[2] = c.v, a.y_page[2] = c.v_page, a.y_slot[2] = c.v_slot, a.y_head[2] = c.v_head;
@@ -360,15 +362,15 @@ extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *c
     return src_dtype == PETB200_F32 ? append_launch<float, __nv_bfloat16>(ctx, a, s) : append_launch<__nv_bfloat16, __nv_bfloat16>(ctx, a, s);
 }
 
-extern "C" int petb200_attention_paged_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, petb200_kv_rows q,
-                                           petb200_kv_rows out, int q_heads, int causal, float scale, void *workspace,
+extern "C" int petb200_attention_paged_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const petb200_kv_rows *q,
+                                           const petb200_kv_rows *out, int q_heads, int causal, float scale, void *workspace,
                                            size_t workspace_bytes, petb200_stream stream) {
     return attention_run(ctx, "attention_paged", cache, seqs, nullptr, 0, q, out, q_heads, causal, scale, workspace, workspace_bytes,
                          (cudaStream_t)stream);
 }
 
 extern "C" int petb200_attention_prefix_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs,
-                                            const int *prefix_table, int prefix_len, petb200_kv_rows q, petb200_kv_rows out, int q_heads,
+                                            const int *prefix_table, int prefix_len, const petb200_kv_rows *q, const petb200_kv_rows *out, int q_heads,
                                             int causal, float scale, void *workspace, size_t workspace_bytes, petb200_stream stream) {
     if (ctx && prefix_len < 0)
         return fail(ctx, PETB200_ERR_INVALID, "attention_prefix: a prefix of %d keys", prefix_len);

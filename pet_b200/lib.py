@@ -5,6 +5,7 @@ The library is the product: importing this module fails loudly when it has not b
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libpetb200.so")
@@ -22,21 +23,14 @@ class TransposeDesc(C.Structure):
     _fields_ = [("split", _i), ("factor", _i), ("ngroups", _i), ("group_sizes", _i * 8), ("flat", _i * 8)]
 
 
-_ll = C.c_longlong
+_b = C.c_char_p  # a descriptor: bytes
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = range(3)
 
 
-class KvCache(C.Structure):
-    _fields_ = [("k", _vp), ("v", _vp), ("k_page", _ll), ("k_slot", _ll), ("k_head", _ll), ("v_page", _ll), ("v_slot", _ll), ("v_head", _ll),
-                ("dtype", _i), ("pages", _i), ("page_size", _i), ("heads", _i), ("dim", _i)]
-
-
-class KvSeqs(C.Structure):
-    _fields_ = [("page_table", _vp), ("kv_lens", _vp), ("q_starts", _vp), ("table_stride", _ll), ("table_width", _i), ("seqs", _i), ("tokens", _i)]
-
-
-class KvRows(C.Structure):
-    _fields_ = [("p", _vp), ("tok", _ll), ("head", _ll)]
+# petb200_kv_cache, petb200_kv_seqs and petb200_kv_rows as bytes (native alignment; the last one pads to eight)
+KV_CACHE = struct.Struct("@PPqqqqqqiiiii4x")
+KV_SEQS = struct.Struct("@PPPqiii4x")
+KV_ROWS = struct.Struct("@Pqq")
 
 
 SYMBOLS = {
@@ -93,10 +87,10 @@ SYMBOLS = {
     "petb200_layernorm_run": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _fp, _vp]),
     "petb200_attention_supported": (_i, [_i, _i, _i, _i]),
     "petb200_attention_run": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
-    "petb200_kv_append_run": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), KvRows, KvRows, KvRows, KvRows, _i, _i, _vp, _i, _i, _i, _vp]),
-    "petb200_attention_paged_run": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), KvRows, KvRows, _i, _i, _fp, _vp, _sz, _vp]),
-    "petb200_attention_prefix_run": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), _vp, _i, KvRows, KvRows, _i, _i, _fp, _vp, _sz, _vp]),
-    "petb200_attention_paged_workspace": (_i, [_vp, C.POINTER(KvCache), C.POINTER(KvSeqs), _i, _i, C.POINTER(_sz)]),
+    "petb200_kv_append_run": (_i, [_vp, _b, _b, _b, _b, _b, _b, _i, _i, _vp, _i, _i, _i, _vp]),
+    "petb200_attention_paged_run": (_i, [_vp, _b, _b, _b, _b, _i, _i, _fp, _vp, _sz, _vp]),
+    "petb200_attention_prefix_run": (_i, [_vp, _b, _b, _vp, _i, _b, _b, _i, _i, _fp, _vp, _sz, _vp]),
+    "petb200_attention_paged_workspace": (_i, [_vp, _b, _b, _i, _i, C.POINTER(_sz)]),
     "petb200_matmul_splitk_noalloc": (_i, [_i] * 7 + [_vp, _vp, _vp, _vp, _i, _vp, C.c_char_p, _sz]),
     "petb200_plan_time": (_i, [_vp, _i, _i, C.POINTER(_fp), _vp]),
 }

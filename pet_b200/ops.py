@@ -16,7 +16,7 @@ from . import lib as L
 # The calls below sit in front of kernels of a few microseconds: plain integers instead of ctypes objects (every entry point
 # declares its argument types), and the stream handle without a torch.cuda.Stream object around it.  torch has these two only
 # where it was built with CUDA; without them the module still imports (shapes, plans' arguments, the graph builders).
-_float32 = torch.float32
+_float32, _int32 = torch.float32, torch.int32
 _KV_TYPES = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
 _current_device, _raw_stream = getattr(torch._C, "_cuda_getDevice", None), getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -80,6 +80,7 @@ class Context:
             raise L.PetError(rc, self.lib.petb200_last_error(None).decode())
         self.device = torch.device("cuda", int(device))
         self._plans = {}
+        self._kv_device, self._kv_need = int(device), {}
 
     def close(self):
         if self.h:
@@ -512,6 +513,8 @@ class Context:
         return y
 
     # ---- paged cache of keys and values --------------------------------------------------------------------
+    # These calls stand in front of kernels of a few microseconds: descriptors are packed as bytes (a fifth of the time that ctypes
+    # structures take), devices compared as numbers, workspace sizes remembered by the sizes they follow from.
     def _kv_stream(self):
         """The current stream of the context's device (which need not be the current one)."""
         if _raw_stream is None:
@@ -519,41 +522,41 @@ class Context:
         return _raw_stream(self.device.index)
 
     def _kv_index(self, name, t, dim):
-        if t.dtype is not torch.int32 or t.dim() != dim or t.device != self.device:
+        if t.dtype is not _int32 or t.dim() != dim or t.get_device() != self._kv_device:
             raise L.PetError(L.ERR_INVALID, f"{name}: an int32 tensor of {dim} dimension(s) on {self.device} expected")
-        return t if t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+        return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
-    def _kv_rows(self, name, t, heads, dim, dtypes, tokens=None):
-        if t.dim() != 3 or t.shape[2] != dim or (heads and t.shape[1] != heads) or (tokens is not None and t.shape[0] != tokens) or \
-                t.dtype not in dtypes or t.device != self.device:
-            raise L.PetError(L.ERR_INVALID, f"{name}: [{tokens if tokens is not None else 'tokens'}, {heads or 'heads'}, {dim}] of the cache's type on "
-                                            f"{self.device} expected, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        return t
-
-    def _kv_aligned(self, t):
-        """Rows as the kernels read them: contiguous in themselves and on the 16-byte grid (a dense copy where a view's are not)."""
-        s0, s1, s2 = t.stride()
-        size = t.element_size()
-        return t if s2 == 1 and not (t.data_ptr() | s0 * size | s1 * size) & 15 else t.clone(memory_format=torch.contiguous_format)
+    def _kv_rows(self, name, t, tokens, heads, dim, dtype):
+        """Strides of rows [tokens, heads (None: any), dim]."""
+        shape = t.shape
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or (heads is not None and shape[1] != heads) or t.dtype is not dtype or \
+                t.get_device() != self._kv_device:
+            raise L.PetError(L.ERR_INVALID, f"{name}: [{tokens}, {'heads' if heads is None else heads}, {dim}] of {dtype} on {self.device} expected, "
+                                            f"got {tuple(shape)} {t.dtype} on {t.device}")
+        return t.stride()
 
     def _kv_call(self, tokens, k_cache, v_cache, page_table, kv_lens, q_starts):
-        """The two descriptions that every call on a cache takes; the last value holds what they point to."""
-        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype not in _KV_TYPES or v_cache.dtype is not k_cache.dtype or \
-                k_cache.device != self.device or v_cache.device != self.device:
+        """The descriptors of the cache and of the sequences that every call takes, heads and dim, sizes that the workspace follows from, and
+        the tensors that the descriptors point to."""
+        shape, dtype = k_cache.shape, k_cache.dtype
+        kind, device = _KV_TYPES.get(dtype), self._kv_device
+        if len(shape) != 4 or shape != v_cache.shape or kind is None or v_cache.dtype is not dtype or k_cache.get_device() != device or \
+                v_cache.get_device() != device:
             raise L.PetError(L.ERR_INVALID, f"k_cache, v_cache: two [pages, page_size, heads, dim] of one type (fp32, fp16, bf16) on {self.device} expected")
-        pages, page_size, heads, dim = k_cache.shape
-        ks, vs = k_cache.stride(), v_cache.stride()
-        if ks[3] != 1 or vs[3] != 1:
+        pages, page_size, heads, dim = shape
+        k_page, k_slot, k_head, k1 = k_cache.stride()
+        v_page, v_slot, v_head, v1 = v_cache.stride()
+        if k1 != 1 or v1 != 1:
             raise L.PetError(L.ERR_UNSUPPORTED, "the values of a head must be contiguous in the cache")
         table, lens = self._kv_index("page_table", page_table, 2), self._kv_index("kv_lens", kv_lens, 1)
+        rows, width = table.shape
         seqs = lens.shape[0]
         starts = None if q_starts is None else self._kv_index("q_starts", q_starts, 1)
-        if table.shape[0] != seqs or (starts is not None and starts.shape[0] != seqs + 1):
+        if rows != seqs or (starts is not None and starts.shape[0] != seqs + 1):
             raise L.PetError(L.ERR_INVALID, f"{seqs} lengths take a page_table of {seqs} rows and {seqs + 1} q_starts")
-        cache = L.KvCache(k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], _KV_TYPES[k_cache.dtype],
-                          pages, page_size, heads, dim)
-        call = L.KvSeqs(table.data_ptr(), lens.data_ptr(), None if starts is None else starts.data_ptr(), table.stride(0), table.shape[1], seqs, tokens)
-        return cache, call, (table, lens, starts)
+        cache = L.KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), k_page, k_slot, k_head, v_page, v_slot, v_head, kind, pages, page_size, heads, dim)
+        call = L.KV_SEQS.pack(table.data_ptr(), lens.data_ptr(), 0 if starts is None else starts.data_ptr(), table.stride(0), width, seqs, tokens)
+        return cache, call, heads, dim, (tokens, seqs, width, kind, pages, page_size, heads, dim, starts is None), (table, lens, starts)
 
     def kv_append(self, k, v, k_cache, v_cache, page_table, kv_lens, q_starts=None, q=None, q_out=None, inv_freq=None, interleaved=False, pos0=0):
         """Writes new tokens' keys and values into a paged cache, keys turned by their positions; returns the turned queries (None without q).
@@ -565,57 +568,81 @@ class Context:
         q_starts[b] .. q_starts[b + 1] - 1 (rows behind the last sequence write nothing); None: as many for each.
         inv_freq [pairs] fp32: pair j is turned by (pos0 + position) * inv_freq[j], the first 2 * pairs values of a head: j with
         j + pairs, or 2 j with 2 j + 1 (interleaved); None: nothing is turned.  No two sequences may append to one page."""
-        cache, call, hold = self._kv_call(k.shape[0], k_cache, v_cache, page_table, kv_lens, q_starts)
-        tokens, heads, dim = k.shape[0], cache.heads, cache.dim
-        types = (k_cache.dtype, _float32)
-        self._kv_rows("k", k, heads, dim, types)
-        self._kv_rows("v", v, heads, dim, (k.dtype,), tokens)
-        rows = []
-        for t in (k, v) if q is None else (k, v, self._kv_rows("q", q, 0, dim, (k.dtype,), tokens)):
-            t = t if t.stride(2) == 1 else t.contiguous()
-            rows.append((t, L.KvRows(t.data_ptr(), t.stride(0), t.stride(1))))
-        q_row = out_row = L.KvRows()
+        tokens = k.shape[0]
+        cache, call, heads, dim, _, hold = self._kv_call(tokens, k_cache, v_cache, page_table, kv_lens, q_starts)
+        dtype, source = k_cache.dtype, k.dtype
+        if source is not dtype and source is not _float32:
+            raise L.PetError(L.ERR_INVALID, f"k, v, q: {dtype} or fp32 expected, got {source}")
+        sk, sv = self._kv_rows("k", k, tokens, heads, dim, source), self._kv_rows("v", v, tokens, heads, dim, source)
+        if sk[2] != 1:
+            k = k.contiguous()
+            sk = k.stride()
+        if sv[2] != 1:
+            v = v.contiguous()
+            sv = v.stride()
+        q_heads, q_rows, out_rows = 0, None, None
         if q is not None:
-            q_row = rows[2][1]
+            sq, q_heads = self._kv_rows("q", q, tokens, None, dim, source), q.shape[1]
+            if sq[2] != 1:
+                q = q.contiguous()
+                sq = q.stride()
             if q_out is None:
-                q_out = torch.empty((tokens, q.shape[1], dim), device=self.device, dtype=k_cache.dtype)
+                q_out = q.new_empty((tokens, q_heads, dim), dtype=dtype)
+                so = (q_heads * dim, dim)
             else:
-                self._kv_rows("q_out", q_out, q.shape[1], dim, (k_cache.dtype,), tokens)
-                if q_out.stride(2) != 1:
+                so = self._kv_rows("q_out", q_out, tokens, q_heads, dim, dtype)
+                if so[2] != 1:
                     raise L.PetError(L.ERR_UNSUPPORTED, "q_out: the values of a head must be contiguous")
-            out_row = L.KvRows(q_out.data_ptr(), q_out.stride(0), q_out.stride(1))
+            q_rows, out_rows = L.KV_ROWS.pack(q.data_ptr(), sq[0], sq[1]), L.KV_ROWS.pack(q_out.data_ptr(), so[0], so[1])
         elif q_out is not None:
             raise L.PetError(L.ERR_INVALID, "q_out without q")
-        pairs = 0
+        pairs, freq = 0, None
         if inv_freq is not None:
-            if inv_freq.dtype is not _float32 or inv_freq.dim() != 1 or inv_freq.device != self.device:
+            if inv_freq.dtype is not _float32 or inv_freq.dim() != 1 or inv_freq.get_device() != self._kv_device:
                 raise L.PetError(L.ERR_INVALID, f"inv_freq: a vector of fp32 on {self.device} expected")
             inv_freq = inv_freq.contiguous()
-            pairs = inv_freq.shape[0]
-        self.check(self.lib.petb200_kv_append_run(self.h, C.byref(cache), C.byref(call), rows[0][1], rows[1][1], q_row, out_row,
-                                                  0 if q is None else q.shape[1], _KV_TYPES[k.dtype], _ptr(inv_freq) if pairs else None, 2 * pairs,
-                                                  int(bool(interleaved)), int(pos0), self._kv_stream()))
+            pairs, freq = inv_freq.shape[0], inv_freq.data_ptr()
+        rc = self.lib.petb200_kv_append_run(self.h, cache, call, L.KV_ROWS.pack(k.data_ptr(), sk[0], sk[1]), L.KV_ROWS.pack(v.data_ptr(), sv[0], sv[1]),
+                                            q_rows, out_rows, q_heads, _KV_TYPES[source], freq, 2 * pairs, 1 if interleaved else 0, pos0, self._kv_stream())
+        if rc:
+            self.check(rc)
         return q_out
 
     def _kv_attention(self, q, k_cache, v_cache, prefix_table, prefix_len, page_table, kv_lens, q_starts, causal, scale, out):
-        cache, call, hold = self._kv_call(q.shape[0], k_cache, v_cache, page_table, kv_lens, q_starts)
-        q = self._kv_aligned(self._kv_rows("q", q, 0, cache.dim, (k_cache.dtype,)))
-        tokens, q_heads = q.shape[0], q.shape[1]
+        tokens = q.shape[0]
+        cache, call, heads, dim, sizes, hold = self._kv_call(tokens, k_cache, v_cache, page_table, kv_lens, q_starts)
+        dtype = k_cache.dtype
+        sq = self._kv_rows("q", q, tokens, None, dim, dtype)
+        q_heads, size = q.shape[1], q.element_size()
+        if sq[2] != 1 or (q.data_ptr() | sq[0] * size | sq[1] * size) & 15:  # rows off the 16-byte grid: a dense copy
+            q = q.clone(memory_format=torch.contiguous_format)
+            sq = q.stride()
         if out is None:
-            out = torch.empty((tokens, q_heads, cache.dim), device=self.device, dtype=q.dtype)
+            out = q.new_empty((tokens, q_heads, dim))
+            so = (q_heads * dim, dim)
         else:
-            self._kv_rows("out", out, q_heads, cache.dim, (q.dtype,), tokens)
-            if out.stride(2) != 1:
+            so = self._kv_rows("out", out, tokens, q_heads, dim, dtype)
+            if so[2] != 1:
                 raise L.PetError(L.ERR_UNSUPPORTED, "out: the values of a head must be contiguous")
-        need = C.c_size_t()
-        self.check(self.lib.petb200_attention_paged_workspace(self.h, C.byref(cache), C.byref(call), prefix_len, q_heads, C.byref(need)))
-        work = torch.empty(need.value, device=self.device, dtype=torch.uint8) if need.value else None
-        rows = L.KvRows(q.data_ptr(), q.stride(0), q.stride(1)), L.KvRows(out.data_ptr(), out.stride(0), out.stride(1))
-        tail = q_heads, int(bool(causal)), cache.dim ** -0.5 if scale is None else float(scale), _ptr(work), need.value, self._kv_stream()
+        sizes += (q_heads, prefix_len)
+        need = self._kv_need.get(sizes)
+        if need is None:
+            n = C.c_size_t()
+            self.check(self.lib.petb200_attention_paged_workspace(self.h, cache, call, prefix_len, q_heads, C.byref(n)))
+            if len(self._kv_need) >= 4096:
+                self._kv_need.clear()
+            need = self._kv_need[sizes] = n.value
+        work = q.new_empty(need, dtype=torch.uint8) if need else None
+        q_rows, out_rows = L.KV_ROWS.pack(q.data_ptr(), sq[0], sq[1]), L.KV_ROWS.pack(out.data_ptr(), so[0], so[1])
+        scale = dim ** -0.5 if scale is None else scale
         if prefix_table is None:
-            self.check(self.lib.petb200_attention_paged_run(self.h, C.byref(cache), C.byref(call), *rows, *tail))
+            rc = self.lib.petb200_attention_paged_run(self.h, cache, call, q_rows, out_rows, q_heads, 1 if causal else 0, scale,
+                                                      work.data_ptr() if need else None, need, self._kv_stream())
         else:
-            self.check(self.lib.petb200_attention_prefix_run(self.h, C.byref(cache), C.byref(call), prefix_table.data_ptr(), prefix_len, *rows, *tail))
+            rc = self.lib.petb200_attention_prefix_run(self.h, cache, call, prefix_table.data_ptr(), prefix_len, q_rows, out_rows, q_heads,
+                                                       1 if causal else 0, scale, work.data_ptr() if need else None, need, self._kv_stream())
+        if rc:
+            self.check(rc)
         return out
 
     def attention_paged(self, q, k_cache, v_cache, page_table, kv_lens, q_starts=None, causal=True, scale=None, out=None):

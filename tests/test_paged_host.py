@@ -15,6 +15,7 @@ class _NoCalls:
 def ctx():
     c = ops.Context.__new__(ops.Context)
     c.lib, c.h, c._plans, c.device = _NoCalls(), None, {}, torch.device("cpu")
+    c._kv_device, c._kv_need = -1, {}  # (what tensors on the host answer)
     return c
 
 
@@ -76,7 +77,32 @@ def test_append_refuses(ctx, change):
 
 def test_entry_points_without_a_context():
     lib = L.load()
-    cache, seqs, rows = L.KvCache(), L.KvSeqs(), L.KvRows()
+    cache, seqs, rows = bytes(L.KV_CACHE.size), bytes(L.KV_SEQS.size), bytes(L.KV_ROWS.size)
     assert lib.petb200_kv_append_run(None, cache, seqs, rows, rows, rows, rows, 0, 0, None, 0, 0, 0, None) == L.ERR_INVALID
     assert lib.petb200_attention_paged_run(None, cache, seqs, rows, rows, 1, 1, 1.0, None, 0, None) == L.ERR_INVALID
     assert lib.petb200_attention_prefix_run(None, cache, seqs, None, 0, rows, rows, 1, 1, 1.0, None, 0, None) == L.ERR_INVALID
+
+
+def test_descriptors_are_packed_as_the_header_lays_them_out(tmp_path):
+    """Sizes and offsets of the C structures, asked of the compiler."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = {"petb200_kv_cache": (L.KV_CACHE, "k v k_page k_slot k_head v_page v_slot v_head dtype pages page_size heads dim"),
+             "petb200_kv_seqs": (L.KV_SEQS, "page_table kv_lens q_starts table_stride table_width seqs tokens"), "petb200_kv_rows": (L.KV_ROWS, "p tok head")}
+    lines = ['#include "petb200.h"', "#include <cstdio>", "#include <cstddef>", "int main() {"]
+    for n, (_, fields) in names.items():
+        lines.append(f'printf("%zu", sizeof({n}));')
+        lines += [f'printf(" %zu", offsetof({n}, {f}));' for f in fields.split()]
+        lines.append('printf("\\n");')
+    src, exe = tmp_path / "o.cc", tmp_path / "o"
+    src.write_text("\n".join(lines) + "\nreturn 0; }\n")
+    subprocess.run(["g++", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.splitlines()
+    for line, (packed, fields) in zip(out, names.values()):
+        size, *offsets = map(int, line.split())
+        assert size == packed.size
+        values = list(range(1, 1 + len(offsets)))
+        blob = packed.pack(*values)
+        for v, o in zip(values, offsets):
+            assert blob[o] == v and blob[o + 1] == 0
