@@ -248,7 +248,8 @@ int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, in
     // Such a sequence gains nothing from the others: its keys, shared and own, are read as one run.
     if (prefix_len == 0 || a.s.seqs == 1 || full)
         return halves && full ? paged_tiles_run(ctx, dtype, a, ws, ws_bytes, need, 0, s) : paged_rows_run(ctx, dtype, a, ws, ws_bytes, need, 0, s);
-    PagedArgs p = a; // all tokens as one sequence that has the shared keys alone
+    // All tokens as one sequence against the shared keys, in pieces; each sequence against its own, as one more piece; the pieces of a row added.
+    PagedArgs p = a;
     p.s.kv_lens = nullptr, p.s.q_starts = nullptr;
     const bool tiles = halves && rows >= kTileFrom;
     int pieces;
@@ -259,21 +260,22 @@ int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, in
         pieces = (int)std::max(1ll, std::min({(2ll * ctx->sm_count + units - 1) / units, (prefix_len + 255ll) / 256, 64ll}));
     }
     const int dp = a.dim > 64 ? 128 : 64;
-    const size_t po = align256((size_t)pieces * a.hkv * rows * dp * 4), pml = align256((size_t)pieces * a.hkv * rows * 8);
+    const size_t po = align256((size_t)(pieces + 1) * a.hkv * rows * dp * 4), pml = align256((size_t)(pieces + 1) * a.hkv * rows * 8);
     p.po = a.po = reinterpret_cast<float *>(ws);
     p.pml = a.pml = reinterpret_cast<float2 *>(ws + po);
+    a.pieces = pieces + 1, a.piece_out = pieces;
     size_t more = 0;
     const bool ask = !a.q;
     if (!ask && po + pml > ws_bytes)
         return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes is too small", ws_bytes);
-    int rc = tiles ? paged_tiles_run(ctx, dtype, p, nullptr, 0, &more, pieces, s) : paged_rows_run(ctx, dtype, p, nullptr, 0, &more, pieces, s);
-    if (rc)
-        return rc;
-    a.s.n0 = 0;
-    a.pieces = pieces;
-    rc = paged_rows_run(ctx, dtype, a, ask ? nullptr : ws + po + pml, ask ? 0 : ws_bytes - po - pml, &more, 0, s);
+    if (tiles) {
+        if (int rc = paged_tiles_run(ctx, dtype, p, nullptr, 0, &more, pieces, s))
+            return rc;
+        a.s.n0 = 0;
+    }
+    int rc = paged_rows_run(ctx, dtype, a, ask ? nullptr : ws + po + pml, ask ? 0 : ws_bytes - po - pml, &more, tiles ? 0 : pieces, s);
     *need = po + pml + more;
-    return rc;
+    return rc || ask ? rc : paged_join_rows(ctx, dtype, a, s);
 }
 
 int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const int *prefix_table,

@@ -73,7 +73,8 @@ struct PagedArgs {
     // m is the largest score * sl2; -inf: the row sees none of these keys, -FLT_MAX: it sees some, all of them at -inf.
     float *po = nullptr;
     float2 *pml = nullptr;
-    int pieces = 0;     // pieces written (this launch) or merged in (po / pml of an earlier launch)
+    int pieces = 0;     // that paged_join_rows() adds
+    int piece_out = -1; // >= 0: results go there as a piece instead of to `out`
     // Split ranges of paged_rows.cu: two pieces and one descriptor per CTA.
     float *ro = nullptr;
     float2 *rml = nullptr;
@@ -100,9 +101,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-int paged_rows_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s);
+// Attention of a's tokens over their keys (and the shared ones before them); *need: the workspace that it takes, all that is done where
+// a.q is NULL.  Where n_prefix > 0, the same launch also forms `n_prefix` pieces of all tokens against a.s.n0 shared keys alone (one
+// sequence of all tokens), and the sequences' own keys go without them.
+int paged_rows_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int n_prefix, cudaStream_t s);
+// The same in 128-row tiles, 16-bit types.  pieces_out > 0: into so many pieces of the keys.
+int paged_tiles_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s);
 // Pieces of the keys that paged_tiles_run() makes of a call by itself.
 int paged_tiles_pieces(petb200_ctx *ctx, const PagedArgs &a);
-int paged_tiles_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s);
+// Adds each row's a.pieces pieces.
+int paged_join_rows(petb200_ctx *ctx, int dtype, const PagedArgs &a, cudaStream_t s);
 
 } // namespace petb200

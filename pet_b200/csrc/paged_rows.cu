@@ -109,6 +109,7 @@ enum { kModeRanges = 0, kModeUnits = 1, kModePieces = 2 };
 // One unit: rows [16 rt, 16 rt + 16) of sequence b's (token, head) pairs on key head h.
 struct Unit {
     int b, rt, h, t0, ql, own, n; // n: keys that its last row sees
+    int skip;                     // shared keys that come before them elsewhere
 };
 
 template <typename T, int DP> struct RowTile {
@@ -127,7 +128,7 @@ template <typename T, int DP> struct RowTile {
         long long ko = -1, vo = 0;
         if (lane < C::CK && base + lane < n) {
             int slot;
-            const int p = a.s.page(u.b, base + lane, slot);
+            const int p = a.s.page(u.b, base + lane + u.skip, slot);
             if (p >= 0) {
                 ko = (long long)p * a.kp + (long long)slot * a.ks + (long long)u.h * a.kh;
                 vo = (long long)p * a.vp + (long long)slot * a.vs + (long long)u.h * a.vh;
@@ -383,7 +384,7 @@ __device__ __forceinline__ void fma4(float4 &x, float w, float4 y) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int mode) {
+__global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int own_mode, int prefix_blocks, int prefix_pieces) {
     using C = RowCfg<T, DP>;
     using Tile = RowTile<T, DP>;
     pdl_prologue();
@@ -395,8 +396,14 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
     const uint32_t ring = ptx::smem_u32(ring_p);
 
     // ---- which steps are this CTA's ------------------------------------------------------------------------------
-    const bool one = a.s.kv_lens == nullptr; // all tokens against the shared keys: a single sequence without keys of its own
-    const int seqs = one ? 1 : a.s.seqs;
+    // The first blocks take all tokens against the shared keys, as a single sequence without keys of its own: unit by unit, each in
+    // pieces.  The others take the sequences.
+    const bool one = (int)blockIdx.x < prefix_blocks;
+    const int mode = one ? kModePieces : own_mode, seqs = one ? 1 : a.s.seqs, n0 = one || prefix_blocks == 0 ? a.s.n0 : 0;
+    const unsigned grid = one ? prefix_blocks / prefix_pieces : gridDim.x - prefix_blocks;
+    const unsigned cta = one ? blockIdx.x / prefix_pieces : blockIdx.x - prefix_blocks;
+    const int piece = one ? (int)(blockIdx.x % prefix_pieces) : a.piece_out;
+    auto visible = [&](int i, int n, int own) { return n0 + (a.causal ? min(max(own - n + i + 1, 0), own) : own); };
     auto tokens_of = [&](int b, int &t0) {
         if (one) {
             t0 = 0;
@@ -404,7 +411,7 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
         }
         return a.s.span(b, t0);
     };
-    auto steps_of = [&](int b) { return mode == kModeRanges ? max(1, (a.s.n0 + a.s.own(b) + C::KT - 1) / C::KT) : 1; };
+    auto steps_of = [&](int b) { return mode == kModeRanges ? max(1, (n0 + a.s.own(b) + C::KT - 1) / C::KT) : 1; };
     auto cost_of = [&](int b) -> unsigned {
         int t0;
         const int tiles = ceil_div(tokens_of(b, t0) * a.group, kRows);
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
         block_scan(b0 + (int)threadIdx.x < seqs ? cost_of(b0 + threadIdx.x) : 0u, t, tmp);
         total += t;
     }
-    const unsigned G = mode == kModeRanges ? min(gridDim.x, total) : total, cta = blockIdx.x;
+    const unsigned G = mode == kModeRanges ? min(grid, total) : total;
     if (mode == kModeRanges && threadIdx.x == 0 && a.meta)
         a.meta[cta] = make_int4(-1, 0, 0, 0);
     if (cta >= G)
@@ -446,22 +453,23 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
         const unsigned steps = steps_of(b), unit = (pos - b_at) / steps, first = (pos - b_at) - unit * steps;
         const unsigned last = min(steps, first + (end - pos));
         Unit u;
+        u.skip = a.s.n0 - n0;
         u.b = b, u.rt = unit / a.hkv, u.h = unit - u.rt * a.hkv;
         u.ql = tokens_of(b, u.t0);
         u.own = one ? 0 : a.s.own(b);
         const int row_end = min((u.rt + 1) * kRows, u.ql * a.group) - 1; // last row of the tile
-        u.n = a.s.visible(row_end / a.group, u.ql, u.own, a.causal);
+        u.n = visible(row_end / a.group, u.ql, u.own);
         // the unit's steps of this CTA as keys
         const int all = (u.n + C::KT - 1) / C::KT;
         int s0 = first, s1 = min((int)last, all);
         if (mode == kModeUnits)
             s0 = 0, s1 = all;
         else if (mode == kModePieces) {
-            s0 = (int)((long long)all * blockIdx.y / gridDim.y), s1 = (int)((long long)all * (blockIdx.y + 1) / gridDim.y);
+            s0 = (int)((long long)all * piece / prefix_pieces), s1 = (int)((long long)all * (piece + 1) / prefix_pieces);
         }
         const int r0 = u.rt * kRows + g, tok0 = r0 / a.group, tok1 = (r0 + 8) / a.group;
-        const int lim0 = tok0 < u.ql ? a.s.visible(tok0, u.ql, u.own, a.causal) : 0, lim1 = tok1 < u.ql ? a.s.visible(tok1, u.ql, u.own, a.causal) : 0;
-        const int full = a.s.visible(u.rt * kRows / a.group, u.ql, u.own, a.causal); // keys that every row sees
+        const int lim0 = tok0 < u.ql ? visible(tok0, u.ql, u.own) : 0, lim1 = tok1 < u.ql ? visible(tok1, u.ql, u.own) : 0;
+        const int full = visible(u.rt * kRows / a.group, u.ql, u.own); // keys that every row sees
 
         Tile tile;
         tile.reset();
@@ -516,32 +524,31 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
             const int row = threadIdx.x >> 3, part = threadIdx.x & 7, rg = u.rt * kRows + row, tok = rg / a.group, hd = rg - tok * a.group;
             if (tok < u.ql) {
                 const bool whole = mode != kModeRanges || (first == 0 && last == steps);
-                const long long grow = (long long)(u.t0 + tok) * a.group + hd, rows = (long long)a.s.tokens * a.group;
-                const int merged = mode != kModePieces && whole ? a.pieces : 0;
                 float M = -INFINITY, L = 0.f, w[kRowWarps];
 #pragma unroll
                 for (int x = 0; x < kRowWarps; ++x) {
                     w[x] = reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * DP * 4)[row].x;
                     M = fmaxf(M, w[x]);
                 }
-                for (int p = 0; p < merged; ++p)
-                    M = fmaxf(M, a.pml[((long long)p * a.hkv + u.h) * rows + grow].x);
 #pragma unroll
                 for (int x = 0; x < kRowWarps; ++x) {
                     w[x] = piece_weight(w[x], M);
                     L += w[x] * reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * DP * 4)[row].y;
                 }
-                for (int p = 0; p < merged; ++p) {
-                    const float2 ml = a.pml[((long long)p * a.hkv + u.h) * rows + grow];
-                    L += piece_weight(ml.x, M) * ml.y;
+                // To `out`; as a piece of the row; or, of a cut unit, as this block's first piece (continued from the block before) or
+                // second (left to the one after).
+                float *po = nullptr;
+                if (!whole) {
+                    const long long at = (long long)(2 * cta + (first > 0 ? 0 : 1)) * kRows + row;
+                    po = a.ro + at * DP;
+                    if (part == 0)
+                        a.rml[at] = make_float2(M, L);
+                } else if (piece >= 0) {
+                    const long long at = ((long long)piece * a.hkv + u.h) * ((long long)a.s.tokens * a.group) + (long long)(u.t0 + tok) * a.group + hd;
+                    po = a.po + at * DP;
+                    if (part == 0)
+                        a.pml[at] = make_float2(M, L);
                 }
-                const int slot = first > 0 ? 0 : 1; // of a cut unit: continued from the CTA before, or left to the one after
-                float *po = mode == kModePieces ? a.po + (((long long)blockIdx.y * a.hkv + u.h) * rows + grow) * DP
-                                                : a.ro + ((long long)(2 * cta + slot) * kRows + row) * DP;
-                if (part == 0 && mode == kModePieces)
-                    a.pml[((long long)blockIdx.y * a.hkv + u.h) * rows + grow] = make_float2(M, L);
-                else if (part == 0 && !whole)
-                    a.rml[(long long)(2 * cta + slot) * kRows + row] = make_float2(M, L);
                 T *out = (T *)a.out + (long long)(u.t0 + tok) * a.o_tok + (long long)(u.h * a.group + hd) * a.o_head;
 #pragma unroll
                 for (int j = 0; j < DP / 32; ++j) {
@@ -550,13 +557,7 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
 #pragma unroll
                     for (int x = 0; x < kRowWarps; ++x)
                         fma4(v, w[x], *reinterpret_cast<const float4 *>(smem + x * C::WARP_BYTES + (row * DP + col) * 4));
-                    for (int p = 0; p < merged; ++p) {
-                        const long long at = ((long long)p * a.hkv + u.h) * rows + grow;
-                        const float f = piece_weight(a.pml[at].x, M);
-                        if (f != 0.f)
-                            fma4(v, f, *reinterpret_cast<const float4 *>(a.po + at * DP + col));
-                    }
-                    if (mode == kModePieces || !whole)
+                    if (po)
                         *reinterpret_cast<float4 *>(po + col) = v;
                     else if (col < a.dim)
                         store4<T>(out + col, settle(v, M, L));
@@ -576,58 +577,111 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
     }
 }
 
-// Adds the pieces of the units that ranges have cut.  A warp per row, four rows per CTA; CTA x looks after the unit that CTA x of the
-// launch before found continued from CTA x - 1, where it began.
-template <typename T, int DP> __global__ void __launch_bounds__(128) k_paged_join(const PagedArgs a) {
+// Sums of a row from n places, a pair of warps sharing them: lane l holds columns 4 l .. 4 l + 3, every second place is the other
+// warp's.  `ml(i)` and `o(i)` say where place i lies.  The loads of eight places are in flight together, since what a row's pieces cost is
+// trips to memory.  Answers in the first warp of the pair.
+template <int DP, typename FM, typename FO> __device__ __forceinline__ void join_pair(int n, FM ml, FO o, float4 *tmp /*[4][32]*/, float (*tml)[2], float4 &v, float &M, float &L) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1, pair = warp >> 1, col = DP == 128 ? lane * 4 : (lane & 15) * 4;
+    M = -INFINITY, L = 0.f;
+    for (int i = lane; i < n; i += 32)
+        M = fmaxf(M, ml(i).x);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1)
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i0 = half; i0 < n; i0 += 16) {
+        float2 w[8];
+        float4 x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = min(i0 + 2 * e, n - 1);
+            w[e] = ml(i);
+            x[e] = *reinterpret_cast<const float4 *>(o(i) + col);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (i0 + 2 * e < n) {
+                const float f = piece_weight(w[e].x, M);
+                L = fmaf(f, w[e].y, L);
+                fma4(v, f, x[e]);
+            }
+    }
+    if (half) {
+        tmp[pair * 32 + lane] = v;
+        tml[pair][0] = L;
+    }
+    __syncthreads();
+    if (!half) {
+        fma4(v, 1.f, tmp[pair * 32 + lane]);
+        L += tml[pair][0];
+    }
+}
+
+// Adds the pieces of the units that ranges have cut, four rows of a unit per CTA; CTA x looks after the unit that CTA x of the launch
+// before found continued from CTA x - 1, where it began.
+template <typename T, int DP> __global__ void __launch_bounds__(256) k_paged_join(const PagedArgs a) {
     pdl_prologue();
+    __shared__ float4 tmp[4 * 32];
+    __shared__ float tml[4][2];
     const int4 d = a.meta[blockIdx.x];
     if (d.x < 0)
         return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 4 + warp;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * 4 + (warp >> 1);
     int t0;
     const int ql = a.s.span(d.x, t0), rg = d.y * kRows + row, tok = rg / a.group, hd = rg - tok * a.group;
-    if (tok >= ql)
-        return;
-    const int c0 = (int)blockIdx.x - 1, n = d.w - c0 + 1;
-    const long long grow = (long long)(t0 + tok) * a.group + hd, rows = (long long)a.s.tokens * a.group;
-    // The unit begins in c0's second piece; where it fills c0 whole, that CTA wrote it as second too (it began there).
+    const int c0 = (int)blockIdx.x - 1, n = tok < ql ? d.w - c0 + 1 : 0;
+    // (the unit is the second piece of the CTA that it begins in, and the first of the others)
     auto place = [&](int i) { return (long long)(2 * (c0 + i) + (i == 0 ? 1 : 0)) * kRows + row; };
-    auto shared = [&](int p) { return ((long long)p * a.hkv + d.z) * rows + grow; };
-    float M = -INFINITY, L = 0.f;
-    for (int i = lane; i < n + a.pieces; i += 32)
-        M = fmaxf(M, (i < n ? a.rml[place(i)] : a.pml[shared(i - n)]).x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 v;
+    float M, L;
+    join_pair<DP>(n, [&](int i) { return a.rml[place(i)]; }, [&](int i) { return a.ro + place(i) * DP; }, tmp, tml, v, M, L);
     const int col = lane * 4;
-#pragma unroll 4
-    for (int i = 0; i < n + a.pieces; ++i) {
-        const long long at = i < n ? place(i) : shared(i - n);
-        const float2 ml = i < n ? a.rml[at] : a.pml[at];
-        const float w = piece_weight(ml.x, M);
-        L += w * ml.y;
-        if (col < DP && w != 0.f)
-            fma4(v, w, *reinterpret_cast<const float4 *>((i < n ? a.ro : a.po) + at * DP + col));
-    }
-    if (col < a.dim)
+    if ((warp & 1) || n == 0 || col >= DP)
+        return;
+    if (a.piece_out >= 0) {
+        const long long at = ((long long)a.piece_out * a.hkv + d.z) * ((long long)a.s.tokens * a.group) + (long long)(t0 + tok) * a.group + hd;
+        *reinterpret_cast<float4 *>(a.po + at * DP + col) = v;
+        if (lane == 0)
+            a.pml[at] = make_float2(M, L);
+    } else if (col < a.dim)
         store4<T>((T *)a.out + (long long)(t0 + tok) * a.o_tok + (long long)(d.z * a.group + hd) * a.o_head + col, settle(v, M, L));
 }
 
+// Adds the pieces of every row, four (token, head) pairs per CTA.
+template <typename T, int DP> __global__ void __launch_bounds__(256) k_paged_join_rows(const PagedArgs a) {
+    pdl_prologue();
+    __shared__ float4 tmp[4 * 32];
+    __shared__ float tml[4][2];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.hkv * a.group;
+    const long long rows = (long long)a.s.tokens * a.group, id = (long long)blockIdx.x * 4 + (warp >> 1);
+    const int tok = (int)(id / heads), head = (int)(id - (long long)tok * heads), h = head / a.group;
+    int n = id < rows * a.hkv ? a.pieces : 0;
+    if (n && a.s.q_starts && (tok < __ldg(a.s.q_starts) || tok >= __ldg(a.s.q_starts + a.s.seqs)))
+        n = 0; // rows outside all sequences stay as they were
+    auto place = [&](int p) { return ((long long)p * a.hkv + h) * rows + (long long)tok * a.group + (head - h * a.group); };
+    float4 v;
+    float M, L;
+    join_pair<DP>(n, [&](int i) { return a.pml[place(i)]; }, [&](int i) { return a.po + place(i) * DP; }, tmp, tml, v, M, L);
+    const int col = lane * 4;
+    if (!(warp & 1) && n && col < a.dim)
+        store4<T>((T *)a.out + (long long)tok * a.o_tok + (long long)head * a.o_head + col, settle(v, M, L));
+}
+
 template <typename T, int DP>
-int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
+int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int n_prefix, cudaStream_t s) {
     using C = RowCfg<T, DP>;
-    const bool one = a.s.kv_lens == nullptr;
+    const long long rows = (long long)a.s.tokens * a.group;
     // Row tiles there can be: a sequence's last one may be short.
-    const long long tiles = one || !a.s.q_starts ? (one ? 1ll : a.s.seqs) * (((long long)(one ? a.s.tokens : a.s.q_len) * a.group + kRows - 1) / kRows)
-                                                 : (long long)a.s.tokens * a.group / kRows + a.s.seqs;
-    const long long units = tiles * a.hkv, keys = (long long)a.s.n0 + (one ? 0 : (long long)a.s.width * a.s.page_size);
-    const long long steps = std::max(1ll, (keys + C::KT - 1) / C::KT);
-    if (keys > 0x7fff0000ll || units * steps > 0x7fff0000ll || (long long)a.s.tokens * a.group > 0x7fff0000ll)
+    const long long tiles = a.s.q_starts ? rows / kRows + a.s.seqs : a.s.seqs * (((long long)a.s.q_len * a.group + kRows - 1) / kRows);
+    const long long units = tiles * a.hkv, own = (long long)a.s.width * a.s.page_size, keys = own + (n_prefix ? 0 : a.s.n0);
+    const long long steps = std::max(1ll, (keys + C::KT - 1) / C::KT), prefix_blocks = (rows + kRows - 1) / kRows * a.hkv * n_prefix;
+    if (own + a.s.n0 > 0x7fff0000ll || units * steps + prefix_blocks > 0x7fff0000ll || rows > 0x7fff0000ll)
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "attention over pages: %lld row tiles of up to %lld keys are more than one call takes", units, keys);
     const int slots = ctx->sm_count * C::CTAS;
-    // Units as they are where there are several rounds of them: ranges would cut each in two for a gain of a part of a round.
-    const int mode = pieces_out ? kModePieces : (units >= 4ll * slots ? kModeUnits : kModeRanges);
+    // Units as they are where there are several rounds of them (ranges would cut each in two for a gain of a part of a round), or
+    // where a unit is a few steps (a second launch would cost more than they).
+    const int mode = units >= 4ll * slots || steps <= 4 ? kModeUnits : kModeRanges;
     const unsigned grid = (unsigned)(mode == kModeRanges ? std::min<long long>(slots, units * steps) : units);
     size_t bytes = 0;
     if (mode == kModeRanges) {
@@ -643,30 +697,48 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
         return PETB200_OK;
     if (bytes > ws_bytes)
         return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes, %zu are needed", ws_bytes, bytes);
-    if (grid == 0)
-        return PETB200_OK;
     if (int rc = raise_smem(ctx, (const void *)k_paged_rows<T, DP>, C::SMEM))
         return rc;
-    launch_pdl(k_paged_rows<T, DP>, dim3(grid, (unsigned)std::max(1, pieces_out)), kRowThreads, C::SMEM, s, a, mode);
+    launch_pdl(k_paged_rows<T, DP>, dim3(grid + (unsigned)prefix_blocks), kRowThreads, C::SMEM, s, a, mode, (int)prefix_blocks, std::max(1, n_prefix));
     int rc = launched(ctx, "k_paged_rows");
     if (rc || mode != kModeRanges)
         return rc;
-    launch_pdl(k_paged_join<T, DP>, dim3(grid, kRows / 4), 128, 0, s, a);
+    // (an even call's tiles have no more rows than its sequences)
+    const int four = (int)std::min<long long>(kRows / 4, a.s.q_starts ? kRows / 4 : ((long long)a.s.q_len * a.group + 3) / 4);
+    launch_pdl(k_paged_join<T, DP>, dim3(grid, (unsigned)four), 256, 0, s, a);
     return launched(ctx, "k_paged_join");
+}
+
+template <typename T, int DP> int join_launch(petb200_ctx *ctx, const PagedArgs &a, cudaStream_t s) {
+    const long long rows = (long long)a.s.tokens * a.group * a.hkv;
+    launch_pdl(k_paged_join_rows<T, DP>, dim3((unsigned)((rows + 3) / 4)), 256, 0, s, a);
+    return launched(ctx, "k_paged_join_rows");
 }
 
 } // namespace
 
-int paged_rows_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
+int paged_rows_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int n_prefix, cudaStream_t s) {
     const bool wide = a.dim > 64;
     switch (dtype) {
     case PETB200_F16:
-        return wide ? rows_launch<__half, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s) : rows_launch<__half, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+        return wide ? rows_launch<__half, 128>(ctx, a, ws, ws_bytes, need, n_prefix, s) : rows_launch<__half, 64>(ctx, a, ws, ws_bytes, need, n_prefix, s);
     case PETB200_BF16:
-        return wide ? rows_launch<__nv_bfloat16, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s)
-                    : rows_launch<__nv_bfloat16, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+        return wide ? rows_launch<__nv_bfloat16, 128>(ctx, a, ws, ws_bytes, need, n_prefix, s)
+                    : rows_launch<__nv_bfloat16, 64>(ctx, a, ws, ws_bytes, need, n_prefix, s);
     default:
-        return wide ? rows_launch<float, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s) : rows_launch<float, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+        return wide ? rows_launch<float, 128>(ctx, a, ws, ws_bytes, need, n_prefix, s) : rows_launch<float, 64>(ctx, a, ws, ws_bytes, need, n_prefix, s);
+    }
+}
+
+int paged_join_rows(petb200_ctx *ctx, int dtype, const PagedArgs &a, cudaStream_t s) {
+    const bool wide = a.dim > 64;
+    switch (dtype) {
+    case PETB200_F16:
+        return wide ? join_launch<__half, 128>(ctx, a, s) : join_launch<__half, 64>(ctx, a, s);
+    case PETB200_BF16:
+        return wide ? join_launch<__nv_bfloat16, 128>(ctx, a, s) : join_launch<__nv_bfloat16, 64>(ctx, a, s);
+    default:
+        return wide ? join_launch<float, 128>(ctx, a, s) : join_launch<float, 64>(ctx, a, s);
     }
 }
 

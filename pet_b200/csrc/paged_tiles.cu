@@ -566,44 +566,6 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
         ptx::tmem_dealloc(tmem, 512);
 }
 
-// Adds the pieces of each row: a warp per (token, head).
-template <typename T, int DP> __global__ void __launch_bounds__(128) k_paged_join_rows(const PagedArgs a) {
-    pdl_prologue();
-    const int lane = threadIdx.x & 31;
-    const long long rows = (long long)a.s.tokens * a.group, id = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (id >= rows * a.hkv)
-        return;
-    const int tok = (int)(id / (a.hkv * a.group)), head = (int)(id - (long long)tok * a.hkv * a.group), h = head / a.group;
-    if (a.s.q_starts) { // rows outside all sequences stay as they were
-        const int first = __ldg(a.s.q_starts), last = __ldg(a.s.q_starts + a.s.seqs);
-        if (tok < first || tok >= last)
-            return;
-    }
-    auto place = [&](int p) { return ((long long)p * a.hkv + h) * rows + (long long)tok * a.group + (head - h * a.group); };
-    float M = -INFINITY, L = 0.f;
-    for (int p = lane; p < a.pieces; p += 32)
-        M = fmaxf(M, a.pml[place(p)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    const int col = lane * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int p = 0; p < a.pieces; ++p) {
-        const float2 ml = a.pml[place(p)];
-        const float w = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - M);
-        L += w * ml.y;
-        if (col < DP && w != 0.f) {
-            const float4 y = *reinterpret_cast<const float4 *>(a.po + place(p) * DP + col);
-            v.x = fmaf(w, y.x, v.x), v.y = fmaf(w, y.y, v.y), v.z = fmaf(w, y.z, v.z), v.w = fmaf(w, y.w, v.w);
-        }
-    }
-    const float f = M == -INFINITY ? 0.f : 1.f / L;
-    if (col < a.dim)
-        *reinterpret_cast<uint2 *>((T *)a.out + (long long)tok * a.o_tok + (long long)head * a.o_head + col) =
-            make_uint2(pack2<T>(v.x * f, v.y * f), pack2<T>(v.z * f, v.w * f));
-}
-
 // The pool as TMA sees it: boxes of up to 128 slots x 64 values of one page and head.  False where the pages do not fit the tiles.
 template <typename T> bool page_map(const PagedArgs &a, const void *pool, long long page, long long slot, long long head, CUtensorMap &map) {
     const int size = a.s.page_size;
@@ -623,7 +585,7 @@ template <typename T> bool page_map(const PagedArgs &a, const void *pool, long l
 }
 
 template <typename T, int DP>
-int tiles_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
+int tiles_launch(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
     using C = TileCfg<DP>;
     const bool one = a.s.kv_lens == nullptr, even = one || !a.s.q_starts;
     const long long rows = (long long)a.s.tokens * a.group;
@@ -655,8 +617,7 @@ int tiles_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_
     int rc = launched(ctx, "k_paged_tiles");
     if (rc || pieces_out || splits == 1)
         return rc;
-    launch_pdl(k_paged_join_rows<T, DP>, dim3((unsigned)((rows * a.hkv + 3) / 4)), 128, 0, s, a);
-    return launched(ctx, "k_paged_join_rows");
+    return paged_join_rows(ctx, dtype, a, s);
 }
 
 } // namespace
@@ -673,9 +634,9 @@ int paged_tiles_pieces(petb200_ctx *ctx, const PagedArgs &a) {
 int paged_tiles_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int pieces_out, cudaStream_t s) {
     const bool wide = a.dim > 64;
     if (dtype == PETB200_F16)
-        return wide ? tiles_launch<__half, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s) : tiles_launch<__half, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
-    return wide ? tiles_launch<__nv_bfloat16, 128>(ctx, a, ws, ws_bytes, need, pieces_out, s)
-                : tiles_launch<__nv_bfloat16, 64>(ctx, a, ws, ws_bytes, need, pieces_out, s);
+        return wide ? tiles_launch<__half, 128>(ctx, dtype, a, ws, ws_bytes, need, pieces_out, s) : tiles_launch<__half, 64>(ctx, dtype, a, ws, ws_bytes, need, pieces_out, s);
+    return wide ? tiles_launch<__nv_bfloat16, 128>(ctx, dtype, a, ws, ws_bytes, need, pieces_out, s)
+                : tiles_launch<__nv_bfloat16, 64>(ctx, dtype, a, ws, ws_bytes, need, pieces_out, s);
 }
 
 } // namespace petb200
