@@ -46,7 +46,7 @@ template <int DP> struct TileCfg {
 static_assert(TileCfg<128>::SMEM <= 227 * 1024, "shared memory of a block");
 
 struct TileCtl {
-    uint64_t q_full, raw, full[8], empty[8], s_full[2], p_full[2], o_full[2]; // raw: a V tile that is looked over before it is full
+    uint64_t q_full, raw, full[8], empty[8], s_full[2], p_full[2][2], o_full[2]; // raw: a V tile that is looked over before it is full
     uint32_t tmem;
     int abort, bad; // bad: non-finite values of V were taken out
     int b, unit;
@@ -87,11 +87,16 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b
     else
         return ptx::pack_bf16x2(a, b);
 }
-// Exponent bits all set in either half.
-template <typename T> __device__ __forceinline__ bool word_bad(uint32_t w) {
-    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    return (w & e) == e || ((w >> 16) & e) == e;
+// 0 * w + c of two 16-bit values: a zero stays one unless a value is not finite
+template <typename T> __device__ __forceinline__ uint32_t zero_times(uint32_t w, uint32_t c) {
+    uint32_t d;
+    if constexpr (std::is_same<T, __half>::value)
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w), "r"(0u), "r"(c));
+    else
+        asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(w), "r"(0u), "r"(c));
+    return d;
 }
+// Values whose exponent bits are all set, taken out
 template <typename T> __device__ __forceinline__ uint32_t word_clean(uint32_t w) {
     constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
     return ((w & e) == e ? 0u : w & 0xffffu) | (((w >> 16) & e) == e ? 0u : w & 0xffff0000u);
@@ -121,14 +126,15 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
         }
         for (int t = 0; t < 2; ++t) {
             ptx::mbar_init(&ctl.s_full[t], 1);
-            ptx::mbar_init(&ctl.p_full[t], 128);
+            ptx::mbar_init(&ctl.p_full[t][0], 128);
+            ptx::mbar_init(&ctl.p_full[t][1], 128);
             ptx::mbar_init(&ctl.o_full[t], 1);
         }
         ctl.abort = ctl.bad = 0;
         ctl.b = -1;
         ptx::fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 15) {
         ptx::tmem_alloc(&ctl.tmem, 512);
         ptx::tmem_relinquish();
     }
@@ -201,30 +207,50 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
             const bool col = piece * 8 < a.dim;
             const T *kc = (const T *)a.kc + (long long)h * a.kh + piece * 8, *vc = (const T *)a.vc + (long long)h * a.vh + piece * 8;
             if (steps > 0) {
-                for (int i = 0; i < tiles * C::NP; ++i) {
-                    const int r = i * C::RP + r0, tok = (row0 + r) / a.group, hd = row0 + r - tok * a.group;
-                    const bool in = col && r < rows;
-                    const T *src = (const T *)a.q + (in ? (long long)(t0 + tok) * a.q_tok + (long long)(h * a.group + hd) * a.q_head + piece * 8 : 0);
-                    cp_async_16_or_zero(q_s + (i / C::NP) * (C::Q / 2) + at0 + (i % C::NP) * (C::RP * 128), src, in ? 16 : 0);
+                // Where each row lies is worked out once, by a thread per row and tile, and read by those that copy its pieces.
+                long long *where = reinterpret_cast<long long *>(row_table);
+                for (int t = 0; t < tiles; ++t) {
+                    const int r = t * kTileRows + lt, tok = (row0 + r) / a.group, hd = row0 + r - tok * a.group;
+                    where[r] = r < rows ? (long long)(t0 + tok) * a.q_tok + (long long)(h * a.group + hd) * a.q_head : -1;
                 }
+                ptx::named_bar_sync(1, 128);
+                for (int t = 0; t < tiles; ++t)
+#pragma unroll 8
+                    for (int i = 0; i < C::NP; ++i) {
+                        const long long at = where[t * kTileRows + i * C::RP + r0];
+                        const bool in = col && at >= 0;
+                        cp_async_16_or_zero(q_s + t * (C::Q / 2) + at0 + i * (C::RP * 128), (const T *)a.q + (in ? at + piece * 8 : 0), in ? 16 : 0);
+                    }
                 asm volatile("cp.async.commit_group;" ::: "memory");
+                ptx::named_bar_sync(1, 128); // (the row table is free)
             }
             // Looks over this thread's pieces of the V tile in stage `st`: rows past the part's end become zeros, non-finite values too
             // where some row does not see some key of the tile (among shared keys every row sees all).
             auto scrub = [&](int j, int st) {
                 unsigned char *p = smem + C::Q + st * C::STAGE + at0;
                 const int left = part_end(j) - first_key(j);
+                if (left < kTileKeys)
+#pragma unroll 1
+                    for (int i = 0; i < C::NP; ++i)
+                        if (i * C::RP + r0 >= left)
+                            *reinterpret_cast<uint4 *>(p + i * (C::RP * 128)) = make_uint4(0u, 0u, 0u, 0u);
+                if (j < tiles0)
+                    return;
+                uint32_t any = 0; // pairs of zeros, or of what 0 x infinity and 0 x NaN give
 #pragma unroll 4
+                for (int i = 0; i < C::NP; ++i) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(p + i * (C::RP * 128));
+                    any = zero_times<T>(x.w, zero_times<T>(x.z, zero_times<T>(x.y, zero_times<T>(x.x, any))));
+                }
+                if ((any & 0x7fff7fffu) == 0)
+                    return;
+#pragma unroll 1
                 for (int i = 0; i < C::NP; ++i) {
                     uint4 *w = reinterpret_cast<uint4 *>(p + i * (C::RP * 128));
                     const uint4 x = *w;
-                    if (i * C::RP + r0 >= left)
-                        *w = make_uint4(0u, 0u, 0u, 0u);
-                    else if (j >= tiles0 && (word_bad<T>(x.x) || word_bad<T>(x.y) || word_bad<T>(x.z) || word_bad<T>(x.w))) {
-                        *w = make_uint4(word_clean<T>(x.x), word_clean<T>(x.y), word_clean<T>(x.z), word_clean<T>(x.w));
-                        *(volatile int *)&ctl.bad = 1;
-                    }
+                    *w = make_uint4(word_clean<T>(x.x), word_clean<T>(x.y), word_clean<T>(x.z), word_clean<T>(x.w));
                 }
+                *(volatile int *)&ctl.bad = 1;
             };
             auto partly = [&](int j) { return first_key(j) + kTileKeys > (j < tiles0 ? n0 : own_first); };
             if (tma) {
@@ -246,14 +272,14 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                     }
                 };
-                if (warp == 8 && steps > 0)
+                if (warp == 10 && steps > 0)
                     look(k0);
                 bool ok = true;
                 int looked = 0; // V tiles looked over so far
                 for (int j = k0; j < k1; ++j) {
                     const bool over = partly(j);
                     const int iv = 2 * (j - k0) + 1, sv = iv % C::NS;
-                    if (warp == 8) {
+                    if (warp == 10) {
                         const int p = page, sl = slot;
                         if (j + 1 < k1)
                             look(j + 1);
@@ -364,15 +390,15 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
         } else if (warp >= 12) {
             ptx::reg_dealloc<kOtherRegs>();
             // ---- products ------------------------------------------------------------------------------------------------
-            if (warp == 12 && steps > 0 && ptx::elect_one()) {
+            if (warp == 15 && steps > 0 && ptx::elect_one()) {
                 const uint32_t kind = std::is_same<T, __half>::value ? ptx::idesc_f16(kTileRows, kTileKeys) : ptx::idesc_bf16(kTileRows, kTileKeys);
                 const uint32_t kind_o = (std::is_same<T, __half>::value ? ptx::idesc_f16(kTileRows, DP) : ptx::idesc_bf16(kTileRows, DP)) | kIdescBMajorMN;
                 auto scores = [&](int t, int s) {
-                    const uint32_t qa = q_s + t * (C::Q / 2), kb = ring + s * C::STAGE;
+                    const uint64_t qa = ptx::smem_desc_k128(q_s + t * (C::Q / 2)), kb = ptx::smem_desc_k128(ring + s * C::STAGE);
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k) {
-                        const uint32_t off = (k >> 2) * (kTileKeys * 128) + (k & 3) * 32;
-                        mma_f16_ss(tmem + t * 128, ptx::smem_desc_k128(qa + off), ptx::smem_desc_k128(kb + off), kind, k > 0);
+                    for (int k = 0; k < DP / 16; ++k) { // (addresses count in 16 bytes)
+                        const uint64_t off = ((k >> 2) * (kTileKeys * 128) + (k & 3) * 32) >> 4;
+                        mma_f16_ss(tmem + t * 128, qa + off, kb + off, kind, k > 0);
                     }
                     ptx::mma_commit(&ctl.s_full[t]);
                 };
@@ -390,14 +416,18 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                     if (ok && more)
                         ok = ptx::mbar_wait(&ctl.full[sk], (ik / C::NS) & 1, abort_flag);
                     for (int t = 0; t < tiles && ok; ++t) {
-                        ok = ptx::mbar_wait(&ctl.p_full[t], j & 1, abort_flag);
+                        const uint64_t vb = smem_desc_mn128(ring + sv * C::STAGE, kTileKeys * 128);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) { // (a half of P is multiplied while the other is being formed)
+                            ok = ok && ptx::mbar_wait(&ctl.p_full[t][half], j & 1, abort_flag);
+                            ptx::tc_fence_after();
+                            if (ok)
+#pragma unroll
+                                for (int k = half * 4; k < half * 4 + 4; ++k)
+                                    ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, vb + k * 128, kind_o, j > 0 || k > 0);
+                        }
                         if (!ok)
                             break;
-                        ptx::tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < kTileKeys / 16; ++k)
-                            ptx::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, smem_desc_mn128(ring + sv * C::STAGE + k * 2048, kTileKeys * 128),
-                                            kind_o, j > 0 || k > 0);
                         if (more)
                             scores(t, sk); // over P, whose product is before it in the pipe
                         else
@@ -485,12 +515,14 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                             p[i] = pack2<T>(x.x, x.y);
                         }
                         ptx::tmem_st_32x16(s_t + c * 16, p);
+                        if (c & 1) {
+                            ptx::tmem_st_wait();
+                            ptx::tc_fence_before();
+                            ptx::mbar_arrive(&ctl.p_full[t][c >> 1]);
+                        }
                     }
                     sum[0] = ptx::add_f32x2(sum[0], sum[1]);
                     l += sum[0].x + sum[0].y;
-                    ptx::tmem_st_wait();
-                    ptx::tc_fence_before();
-                    ptx::mbar_arrive(&ctl.p_full[t]);
                 }
                 // ---- the rows' results --------------------------------------------------------------------------------------
                 if (ok && steps > 0)
@@ -562,7 +594,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
     }
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 12)
+    if (warp == 15)
         ptx::tmem_dealloc(tmem, 512);
 }
 
