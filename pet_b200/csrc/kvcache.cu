@@ -98,58 +98,99 @@ template <typename S, typename T> __global__ void __launch_bounds__(kAppendThrea
         turn[t][j] = make_float2(cs, sn);
     }
     __syncthreads();
-    const int per_head = a.dim / 8, heads = a.heads[0] + a.heads[1] + a.heads[2], pieces = heads * per_head;
-    for (int i = blockIdx.y * kAppendThreads + threadIdx.x; i < ntok * pieces; i += gridDim.y * kAppendThreads) {
-        const int t = i / pieces, r = i - t * pieces, hh = r / per_head, d = (r - hh * per_head) * 8;
-        const int kind = hh < a.heads[0] ? 0 : hh < a.heads[0] + a.heads[1] ? 1 : 2;
-        const int h = hh - (kind > 0 ? a.heads[0] : 0) - (kind > 1 ? a.heads[1] : 0);
-        const int page = where[t][0];
-        if (kind ? page < 0 : !where[t][2])
-            continue;
-        const S *x = (const S *)a.x[kind] + (long long)(tok0 + t) * a.x_tok[kind] + (long long)h * a.x_head[kind];
-        float v[8];
-        load8(x + d, a.vec, v);
-        if (kind < 2 && d < a.rot) {
-            if (a.interleaved) {
+    // A thread takes two 16-byte pieces of a head at a time, so that the halves of a pair are read once: pieces d and d + half where
+    // that is how values pair up, neighbours elsewhere (values, interleaved pairs, what is not turned).  Eight threads or fewer share
+    // a head of 128; `step` (token, head) pairs are walked at once, two rounds of loads ahead of their stores.
+    const int per_head = (a.dim + 15) / 16, group = threadIdx.x / per_head, step = kAppendThreads / per_head, e = threadIdx.x - group * per_head;
+    const int heads = a.heads[0] + a.heads[1] + a.heads[2], turned = a.interleaved || (half & 7) ? 0 : half / 8; // piece pairs that are halves
+    if (group >= step)
+        return;
+    struct Two {
+        float v[2][8];
+        const S *x; // the head's values
+        T *y;       // where they go; null: nowhere
+        int d[2], t, kind;
+    };
+    auto fetch = [&](int i, Two &w) {
+        const int t = i / heads, hh = i - t * heads;
+        w.y = nullptr;
+        if (t >= ntok)
+            return;
+        w.kind = hh < a.heads[0] ? 0 : hh < a.heads[0] + a.heads[1] ? 1 : 2, w.t = t;
+        const int h = hh - (w.kind > 0 ? a.heads[0] : 0) - (w.kind > 1 ? a.heads[1] : 0), page = where[t][0];
+        if (w.kind ? page < 0 : !where[t][2])
+            return;
+        if (w.kind < 2 && turned)
+            w.d[0] = e < turned ? e * 8 : a.rot + (e - turned) * 16, w.d[1] = w.d[0] + (e < turned ? half : 8);
+        else
+            w.d[0] = e * 16, w.d[1] = e * 16 + 8;
+        w.x = (const S *)a.x[w.kind] + (long long)(tok0 + t) * a.x_tok[w.kind] + (long long)h * a.x_head[w.kind];
 #pragma unroll
-                for (int e = 0; e < 8; e += 2)
-                    if (d + e < a.rot) {
-                        const float2 c = turn[t][(d + e) >> 1];
-                        const float x1 = v[e], x2 = v[e + 1];
-                        v[e] = x1 * c.x - x2 * c.y, v[e + 1] = x2 * c.x + x1 * c.y;
+        for (int k = 0; k < 2; ++k)
+            if (w.d[k] < a.dim)
+                load8(w.x + w.d[k], a.vec, w.v[k]);
+        w.y = (T *)a.y[w.kind] + (long long)h * a.y_head[w.kind] +
+              (w.kind ? (long long)page * a.y_page[w.kind] + (long long)where[t][1] * a.y_slot[w.kind] : (long long)(tok0 + t) * a.y_tok);
+    };
+    auto put = [&](Two &w) {
+        if (!w.y)
+            return;
+        if (w.kind < 2) {
+            const float2 *c = turn[w.t];
+            if (turned) {
+                if (e < turned)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 cs = c[e * 8 + k];
+                        const float x1 = w.v[0][k], x2 = w.v[1][k];
+                        w.v[0][k] = x1 * cs.x - x2 * cs.y, w.v[1][k] = x2 * cs.x + x1 * cs.y;
                     }
-            } else if ((half & 7) == 0) { // the other halves of the pairs are a piece too
-                float o[8];
-                const bool low = d < half;
-                load8(x + (low ? d + half : d - half), a.vec, o);
+            } else if (a.interleaved) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float2 c = turn[t][low ? d + e : d + e - half];
-                    v[e] = low ? v[e] * c.x - o[e] * c.y : v[e] * c.x + o[e] * c.y;
-                }
-            } else {
+                for (int p = 0; p < 2; ++p)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (d + e < a.rot) {
-                        const bool low = d + e < half;
-                        const float2 c = turn[t][low ? d + e : d + e - half];
-                        const float o = to_f32(x[low ? d + e + half : d + e - half]);
-                        v[e] = low ? v[e] * c.x - o * c.y : v[e] * c.x + o * c.y;
+                    for (int k = 0; k < 8; k += 2)
+                        if (w.d[p] + k < a.rot) {
+                            const float2 cs = c[(w.d[p] + k) >> 1];
+                            const float x1 = w.v[p][k], x2 = w.v[p][k + 1];
+                            w.v[p][k] = x1 * cs.x - x2 * cs.y, w.v[p][k + 1] = x2 * cs.x + x1 * cs.y;
+                        }
+            } else { // halves that do not fall on pieces: the other value of each pair is read by itself
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int d = w.d[p] + k;
+                        if (d < a.rot) {
+                            const bool low = d < half;
+                            const float2 cs = c[low ? d : d - half];
+                            const float o = to_f32(w.x[low ? d + half : d - half]);
+                            w.v[p][k] = low ? w.v[p][k] * cs.x - o * cs.y : w.v[p][k] * cs.x + o * cs.y;
+                        }
                     }
             }
         }
-        T *y = (T *)a.y[kind] + (long long)h * a.y_head[kind] + d;
-        y += kind ? (long long)page * a.y_page[kind] + (long long)where[t][1] * a.y_slot[kind] : (long long)(tok0 + t) * a.y_tok;
-        store8(y, v);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (w.d[k] < a.dim)
+                store8(w.y + w.d[k], w.v[k]);
+    };
+    const int all = ntok * heads;
+    for (int i = blockIdx.y * step + group; i < all; i += 2 * gridDim.y * step) {
+        Two p, q;
+        fetch(i, p);
+        fetch(i + gridDim.y * step, q);
+        put(p);
+        put(q);
     }
 }
 
 template <typename S, typename T> int append_launch(petb200_ctx *ctx, AppendArgs &a, cudaStream_t s) {
-    const int pieces = (a.heads[0] + a.heads[1] + a.heads[2]) * (a.dim / 8);
-    // Several tokens to a block share its angles and barriers; few tokens are spread over blocks instead, one piece a thread.
+    const int heads = a.heads[0] + a.heads[1] + a.heads[2], step = kAppendThreads / ((a.dim + 15) / 16);
+    // Several tokens to a block share its angles and barriers; few tokens are spread over blocks instead, a head or two a thread.
     a.tokens_per_block = a.s.tokens >= kAppendTokens * 2 * ctx->sm_count ? kAppendTokens : 1;
     const int blocks = ceil_div(a.s.tokens, a.tokens_per_block);
-    const int split = blocks < 4 * ctx->sm_count ? std::min(ceil_div(pieces, kAppendThreads), 64) : 1;
+    const int split = blocks < 4 * ctx->sm_count ? std::min(ceil_div(heads, step), 64) : 1;
     launch_pdl(k_kv_append<S, T>, dim3((unsigned)blocks, (unsigned)split), kAppendThreads, 0, s, a);
     return launched(ctx, "k_kv_append");
 }

@@ -583,22 +583,30 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
 template <int DP, typename FM, typename FO> __device__ __forceinline__ void join_pair(int n, FM ml, FO o, float4 *tmp /*[4][32]*/, float (*tml)[2], float4 &v, float &M, float &L) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1, pair = warp >> 1, col = DP == 128 ? lane * 4 : (lane & 15) * 4;
     M = -INFINITY, L = 0.f;
-    for (int i = lane; i < n; i += 32)
-        M = fmaxf(M, ml(i).x);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1)
-        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
     v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
-    for (int i0 = half; i0 < n; i0 += 16) {
-        float2 w[8];
-        float4 x[8];
+    float2 w[8];
+    float4 x[8];
+    auto load = [&](int i0) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int i = min(i0 + 2 * e, n - 1);
-            w[e] = ml(i);
-            x[e] = *reinterpret_cast<const float4 *>(o(i) + col);
+            if (e < 1 || i0 + 2 * e < n) {
+                w[e] = ml(i);
+                x[e] = *reinterpret_cast<const float4 *>(o(i) + col);
+            }
         }
+    };
+    if (half < n)
+        load(half); // (with the maxima: the first sixteen places are one trip)
+    for (int i = lane; i < n; i += 32)
+        M = fmaxf(M, ml(i).x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+        M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+#pragma unroll 1
+    for (int i0 = half; i0 < n; i0 += 16) {
+        if (i0 != half)
+            load(i0);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             if (i0 + 2 * e < n) {
