@@ -37,11 +37,14 @@ template <typename T, int DP> struct RowCfg {
     static constexpr int RPI = 32 / CPR;                    // rows that one copy instruction of the warp covers
     static constexpr int NI = CK / RPI;                     // copy instructions per operand and step
     static constexpr int HALF = CK * DP * (int)sizeof(T);   // bytes of one operand's stage
-    static constexpr int NST = DP == 128 ? 3 : 4;           // stages
+    // Blocks per SM, and stages of a warp's ring: three blocks of two stages at 168 registers a thread, or two of three at 255, take the
+    // same time over long sequences (184 us for 64 of up to 8000 keys); short ones gain from the third block (128 of up to 500 keys behind
+    // a prefix: 117 -> 114 us).  fp32's hi and lo queries of 128 values spill at 168.
+    static constexpr int CTAS = DP == 128 && f32 ? 2 : 3, NST = DP == 64 ? 4 : f32 ? 3 : 2;
+    static constexpr int MP = DP + 8;                       // pitch of a row of sums where the warps meet: eight rows, eight banks
     static constexpr int WARP_BYTES = 2 * HALF * NST;
     static constexpr int SMEM = WARP_BYTES * kRowWarps;
-    static constexpr int CTAS = DP == 128 ? 2 : 3;          // per SM, by shared memory
-    static_assert(WARP_BYTES >= kRows * (DP + 2) * 4, "a warp's stages hold its accumulators when the warps meet");
+    static_assert(WARP_BYTES >= kRows * (MP + 2) * 4, "a warp's stages hold its accumulators when the warps meet");
     static_assert(SMEM * CTAS <= 224 * 1024, "shared memory of an SM");
 };
 
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
 
         // ---- the warps meet: {m, l} and O of each in its own stages --------------------------------------------------
         float *wo = reinterpret_cast<float *>(ring_p);
-        float2 *wm = reinterpret_cast<float2 *>(wo + kRows * DP);
+        float2 *wm = reinterpret_cast<float2 *>(wo + kRows * C::MP);
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             float l = tile.l[r];
@@ -514,11 +517,20 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
             if ((lane & 3) == 0)
                 wm[g + 8 * r] = make_float2(seen ? fmaxf(tile.m[r], -FLT_MAX) : -INFINITY, l);
         }
+        if constexpr (C::f32) {
 #pragma unroll
-        for (int t = 0; t < DP / 8; ++t)
+            for (int t = 0; t < DP / 8; t += 4)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                wo[(g + 8 * (e >> 1)) * DP + Tile::column(t, e)] = tile.o[t][e];
+                for (int e = 0; e < 4; ++e)
+                    *reinterpret_cast<float4 *>(&wo[(g + 8 * (e >> 1)) * C::MP + Tile::column(t, e)]) =
+                        make_float4(tile.o[t][e], tile.o[t + 1][e], tile.o[t + 2][e], tile.o[t + 3][e]);
+        } else {
+#pragma unroll
+            for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    *reinterpret_cast<float2 *>(&wo[(g + 8 * r) * C::MP + Tile::column(t, 0)]) = make_float2(tile.o[t][2 * r], tile.o[t][2 * r + 1]);
+        }
         __syncthreads();
         {
             const int row = threadIdx.x >> 3, part = threadIdx.x & 7, rg = u.rt * kRows + row, tok = rg / a.group, hd = rg - tok * a.group;
@@ -527,13 +539,13 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
                 float M = -INFINITY, L = 0.f, w[kRowWarps];
 #pragma unroll
                 for (int x = 0; x < kRowWarps; ++x) {
-                    w[x] = reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * DP * 4)[row].x;
+                    w[x] = reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * C::MP * 4)[row].x;
                     M = fmaxf(M, w[x]);
                 }
 #pragma unroll
                 for (int x = 0; x < kRowWarps; ++x) {
                     w[x] = piece_weight(w[x], M);
-                    L += w[x] * reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * DP * 4)[row].y;
+                    L += w[x] * reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * C::MP * 4)[row].y;
                 }
                 // To `out`; as a piece of the row; or, of a cut unit, as this block's first piece (continued from the block before) or
                 // second (left to the one after).
@@ -556,7 +568,7 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
                     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                     for (int x = 0; x < kRowWarps; ++x)
-                        fma4(v, w[x], *reinterpret_cast<const float4 *>(smem + x * C::WARP_BYTES + (row * DP + col) * 4));
+                        fma4(v, w[x], *reinterpret_cast<const float4 *>(smem + x * C::WARP_BYTES + (row * C::MP + col) * 4));
                     if (po)
                         *reinterpret_cast<float4 *>(po + col) = v;
                     else if (col < a.dim)
