@@ -118,7 +118,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
     }
 
     if (threadIdx.x == 0) {
-        ptx::mbar_init(&ctl.q_full, 128);
+        ptx::mbar_init(&ctl.q_full, tma ? 96 : 128);
         ptx::mbar_init(&ctl.raw, 1);
         for (int i = 0; i < C::NS; ++i) {
             ptx::mbar_init(&ctl.full[i], tma ? 1 : 128);
@@ -160,14 +160,16 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
     const int split = blockIdx.x % splits, place = blockIdx.x / splits;
     if (warp == 0) { // units are laid end to end and taken from the last one down: later rows of a prompt see more keys
         const int seqs = one ? 1 : a.s.seqs;
-        unsigned total = 0;
-        for (int b0 = 0; b0 < seqs; b0 += 32)
-            total += __reduce_add_sync(0xffffffffu, b0 + lane < seqs ? (unsigned)units_of(b0 + lane) : 0u);
+        auto count = [&](int b0) { return b0 + lane < seqs ? (unsigned)units_of(b0 + lane) : 0u; };
+        unsigned c = count(0), total = __reduce_add_sync(0xffffffffu, c);
+        for (int b0 = 32; b0 < seqs; b0 += 32)
+            total += __reduce_add_sync(0xffffffffu, count(b0));
         if ((unsigned)place < total) {
             const unsigned mine = total - 1 - place;
             unsigned run = 0;
             for (int b0 = 0; b0 < seqs && run <= mine; b0 += 32) {
-                const unsigned c = b0 + lane < seqs ? (unsigned)units_of(b0 + lane) : 0u;
+                if (b0 > 0)
+                    c = count(b0);
                 unsigned inc = c;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -206,24 +208,25 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
             const uint32_t at0 = (uint32_t)((piece >> 3) * (kTileKeys * 128) + r0 * 128 + (((piece & 7) ^ (r0 & 7)) << 4)); // (rows of a thread agree in r & 7)
             const bool col = piece * 8 < a.dim;
             const T *kc = (const T *)a.kc + (long long)h * a.kh + piece * 8, *vc = (const T *)a.vc + (long long)h * a.vh + piece * 8;
-            if (steps > 0) {
-                // Where each row lies is worked out once, by a thread per row and tile, and read by those that copy its pieces.
+            // The query rows, by `count` threads of which this is the `me`-th.  Where each row lies is worked out once, by one of them.
+            auto fetch_q = [&](int me, int count) {
                 long long *where = reinterpret_cast<long long *>(row_table);
-                for (int t = 0; t < tiles; ++t) {
-                    const int r = t * kTileRows + lt, tok = (row0 + r) / a.group, hd = row0 + r - tok * a.group;
+#pragma unroll 1
+                for (int r = me; r < tiles * kTileRows; r += count) {
+                    const int tok = (row0 + r) / a.group, hd = row0 + r - tok * a.group;
                     where[r] = r < rows ? (long long)(t0 + tok) * a.q_tok + (long long)(h * a.group + hd) * a.q_head : -1;
                 }
-                ptx::named_bar_sync(1, 128);
-                for (int t = 0; t < tiles; ++t)
-#pragma unroll 8
-                    for (int i = 0; i < C::NP; ++i) {
-                        const long long at = where[t * kTileRows + i * C::RP + r0];
-                        const bool in = col && at >= 0;
-                        cp_async_16_or_zero(q_s + t * (C::Q / 2) + at0 + i * (C::RP * 128), (const T *)a.q + (in ? at + piece * 8 : 0), in ? 16 : 0);
-                    }
+                ptx::named_bar_sync(2, count);
+#pragma unroll 4
+                for (int i = me; i < tiles * kTileRows * C::CPR; i += count) {
+                    const int r = i / C::CPR, c = i % C::CPR;
+                    const long long at = where[r];
+                    const bool in = c * 8 < a.dim && at >= 0;
+                    cp_async_16_or_zero(q_s + (r >> 7) * (C::Q / 2) + (c >> 3) * (kTileRows * 128) + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                        (const T *)a.q + (in ? at + c * 8 : 0), in ? 16 : 0);
+                }
                 asm volatile("cp.async.commit_group;" ::: "memory");
-                ptx::named_bar_sync(1, 128); // (the row table is free)
-            }
+            };
             // Looks over this thread's pieces of the V tile in stage `st`: rows past the part's end become zeros, non-finite values too
             // where some row does not see some key of the tile (among shared keys every row sees all).
             auto scrub = [&](int j, int st) {
@@ -254,10 +257,12 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
             };
             auto partly = [&](int j) { return first_key(j) + kTileKeys > (j < tiles0 ? n0 : own_first); };
             if (tma) {
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                ptx::fence_proxy_async_smem();
-                if (steps > 0)
+                if (warp != 10 && steps > 0) { // (one warp goes ahead with the keys)
+                    fetch_q(warp < 10 ? lt : lt - 32, 96);
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    ptx::fence_proxy_async_smem();
                     ptx::mbar_arrive(&ctl.q_full);
+                }
                 const int box = min(a.s.page_size, kTileKeys), boxes = kTileKeys / box, sub = lane % C::SUBS, mine = lane / C::SUBS;
                 // A lane looks up the page of its box, a tile ahead.  No page (past the keys, or not one): a page past the last, zeros.
                 int page = 0, slot = 0;
@@ -315,6 +320,10 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                     }
                 }
             } else {
+                if (steps > 0) {
+                    fetch_q(lt, 128);
+                    ptx::named_bar_sync(1, 128); // (the row table is free)
+                }
                 int issued = steps > 0 ? 1 : 0, told = 0; // of Q, K 0, V 0, K 1, ...
                 auto tell = [&]() {                      // the oldest of them has arrived: its own copies, then everyone's
                     if (told > 0 && !(told & 1)) {
