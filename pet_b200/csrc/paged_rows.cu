@@ -107,7 +107,7 @@ __device__ __forceinline__ unsigned block_scan(unsigned x, unsigned &total, unsi
     return before + inc - x;
 }
 
-enum { kModeRanges = 0, kModeUnits = 1, kModePieces = 2 };
+enum { kModeRanges = 0, kModeUnits = 1, kModePieces = 2, kModeCluster = 3 };
 
 // One unit: rows [16 rt, 16 rt + 16) of sequence b's (token, head) pairs on key head h.
 struct Unit {
@@ -387,12 +387,13 @@ __device__ __forceinline__ void fma4(float4 &x, float w, float4 y) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int own_mode, int prefix_blocks, int prefix_pieces) {
+__global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int own_mode, int prefix_blocks, int prefix_pieces, int cluster) {
     using C = RowCfg<T, DP>;
     using Tile = RowTile<T, DP>;
     pdl_prologue();
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ unsigned tmp[kRowWarps];
+    __shared__ float2 joined[kRows]; // {m, l} of the block's rows, for its cluster
     __shared__ unsigned found[2]; // sequence that holds this CTA's first step, and where it begins
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     unsigned char *ring_p = smem + warp * C::WARP_BYTES;
@@ -404,7 +405,9 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
     const bool one = (int)blockIdx.x < prefix_blocks;
     const int mode = one ? kModePieces : own_mode, seqs = one ? 1 : a.s.seqs, n0 = one || prefix_blocks == 0 ? a.s.n0 : 0;
     const unsigned grid = one ? prefix_blocks / prefix_pieces : gridDim.x - prefix_blocks;
-    const unsigned cta = one ? blockIdx.x / prefix_pieces : blockIdx.x - prefix_blocks;
+    // (a unit's share of the cluster: all blocks of a cluster have one unit, and leave or stay together)
+    const unsigned cta = one ? blockIdx.x / prefix_pieces : mode == kModeCluster ? blockIdx.x / cluster : blockIdx.x - prefix_blocks;
+    const int rank = mode == kModeCluster ? (int)(blockIdx.x % cluster) : 0;
     const int piece = one ? (int)(blockIdx.x % prefix_pieces) : a.piece_out;
     auto visible = [&](int i, int n, int own) { return n0 + (a.causal ? min(max(own - n + i + 1, 0), own) : own); };
     auto tokens_of = [&](int b, int &t0) {
@@ -467,7 +470,9 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
         int s0 = first, s1 = min((int)last, all);
         if (mode == kModeUnits)
             s0 = 0, s1 = all;
-        else if (mode == kModePieces) {
+        else if (mode == kModeCluster) {
+            s0 = (int)((long long)all * rank / cluster), s1 = (int)((long long)all * (rank + 1) / cluster);
+        } else if (mode == kModePieces) {
             s0 = (int)((long long)all * piece / prefix_pieces), s1 = (int)((long long)all * (piece + 1) / prefix_pieces);
         }
         const int r0 = u.rt * kRows + g, tok0 = r0 / a.group, tok1 = (r0 + 8) / a.group;
@@ -548,9 +553,10 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
                     L += w[x] * reinterpret_cast<const float2 *>(smem + x * C::WARP_BYTES + kRows * C::MP * 4)[row].y;
                 }
                 // To `out`; as a piece of the row; or, of a cut unit, as this block's first piece (continued from the block before) or
-                // second (left to the one after).
+                // second (left to the one after); or to the cluster.
                 float *po = nullptr;
-                if (!whole) {
+                if (mode == kModeCluster) {
+                } else if (!whole) {
                     const long long at = (long long)(2 * cta + (first > 0 ? 0 : 1)) * kRows + row;
                     po = a.ro + at * DP;
                     if (part == 0)
@@ -569,11 +575,41 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
 #pragma unroll
                     for (int x = 0; x < kRowWarps; ++x)
                         fma4(v, w[x], *reinterpret_cast<const float4 *>(smem + x * C::WARP_BYTES + (row * C::MP + col) * 4));
-                    if (po)
+                    if (mode == kModeCluster) // (over the first warp's sums: nobody but this thread reads these)
+                        *reinterpret_cast<float4 *>(smem + (row * C::MP + col) * 4) = v;
+                    else if (po)
                         *reinterpret_cast<float4 *>(po + col) = v;
                     else if (col < a.dim)
                         store4<T>(out + col, settle(v, M, L));
                 }
+                if (mode == kModeCluster && part == 0)
+                    joined[row] = make_float2(M, L);
+            }
+            if (mode == kModeCluster) {
+                // The blocks of the cluster add their sums, each a share of the rows, from one another's shared memory.
+                ptx::cluster_sync_all();
+                constexpr int TPR = DP / 4; // threads of a row, four columns each
+                for (int rr = rank + cluster * (int)(threadIdx.x / TPR); rr < kRows; rr += cluster * (kRowThreads / TPR)) {
+                    const int rg2 = u.rt * kRows + rr, tok2 = rg2 / a.group, hd2 = rg2 - tok2 * a.group, col = (int)(threadIdx.x % TPR) * 4;
+                    if (tok2 >= u.ql)
+                        continue;
+                    const uint32_t at_ml = ptx::smem_u32(&joined[rr]), at_o = ptx::smem_u32(smem + (rr * C::MP + col) * 4);
+                    float M = -INFINITY, L = 0.f;
+                    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (int p = 0; p < cluster; ++p)
+                        M = fmaxf(M, ptx::ld_dsmem_f32(ptx::map_to_cta(at_ml, p)));
+#pragma unroll 4
+                    for (int p = 0; p < cluster; ++p) {
+                        const uint32_t m_at = ptx::map_to_cta(at_ml, p), o_at = ptx::map_to_cta(at_o, p);
+                        const float f = piece_weight(ptx::ld_dsmem_f32(m_at), M);
+                        L = fmaf(f, ptx::ld_dsmem_f32(m_at + 4), L);
+                        fma4(v, f, make_float4(ptx::ld_dsmem_f32(o_at), ptx::ld_dsmem_f32(o_at + 4), ptx::ld_dsmem_f32(o_at + 8), ptx::ld_dsmem_f32(o_at + 12)));
+                    }
+                    if (col < a.dim)
+                        store4<T>((T *)a.out + (long long)(u.t0 + tok2) * a.o_tok + (long long)(u.h * a.group + hd2) * a.o_head + col, settle(v, M, L));
+                }
+                ptx::cluster_sync_all(); // (a block's shared memory stays until the others have read it)
             }
             if (mode == kModeRanges && first > 0 && threadIdx.x == 0) {
                 // The first CTA after the one in which the unit begins says where its pieces are.
@@ -701,8 +737,11 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
     const int slots = ctx->sm_count * C::CTAS;
     // Units as they are where there are several rounds of them (ranges would cut each in two for a gain of a part of a round), or
     // where a unit is a few steps (a second launch would cost more than they).
-    const int mode = units >= 4ll * slots || steps <= 4 ? kModeUnits : kModeRanges;
-    const unsigned grid = (unsigned)(mode == kModeRanges ? std::min<long long>(slots, units * steps) : units);
+    // Few units of moderate length go to a cluster of blocks each, which add their sums through shared memory: one launch and no
+    // workspace (one token on 1500 keys, 8 units: 15.5 us a call with ranges, whose second launch alone costs the host 2.5).
+    const int cluster = n_prefix || a.piece_out >= 0 || steps <= 4 ? 0 : units * 8 <= slots && steps <= 64 ? 8 : units * 4 <= slots && steps <= 32 ? 4 : 0;
+    const int mode = cluster ? kModeCluster : units >= 4ll * slots || steps <= 4 ? kModeUnits : kModeRanges;
+    const unsigned grid = (unsigned)(mode == kModeRanges ? std::min<long long>(slots, units * steps) : mode == kModeCluster ? units * cluster : units);
     size_t bytes = 0;
     if (mode == kModeRanges) {
         a.ro = reinterpret_cast<float *>(ws);
@@ -719,7 +758,19 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
         return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes, %zu are needed", ws_bytes, bytes);
     if (int rc = raise_smem(ctx, (const void *)k_paged_rows<T, DP>, C::SMEM))
         return rc;
-    launch_pdl(k_paged_rows<T, DP>, dim3(grid + (unsigned)prefix_blocks), kRowThreads, C::SMEM, s, a, mode, (int)prefix_blocks, std::max(1, n_prefix));
+    if (mode == kModeCluster) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(grid), cfg.blockDim = dim3(kRowThreads), cfg.dynamicSmemBytes = C::SMEM, cfg.stream = s;
+        cudaLaunchAttribute attr[2]{};
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        (void)cudaLaunchKernelEx(&cfg, k_paged_rows<T, DP>, a, mode, 0, 1, cluster);
+        return launched(ctx, "k_paged_rows");
+    }
+    launch_pdl(k_paged_rows<T, DP>, dim3(grid + (unsigned)prefix_blocks), kRowThreads, C::SMEM, s, a, mode, (int)prefix_blocks, std::max(1, n_prefix), 1);
     int rc = launched(ctx, "k_paged_rows");
     if (rc || mode != kModeRanges)
         return rc;

@@ -152,6 +152,21 @@ def test_long_sequences_among_short_ones(ctx, dtype):
     c.check(c.attend(ctx))
 
 
+# Few sequences on a cluster of eight blocks each, more on four, more on ranges: keys that leave some blocks of a cluster without any, none at all
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("seqs", [1, 20, 40, 80])
+@pytest.mark.parametrize("dim", [64, 104])
+def test_sequences_that_share_the_gpu(ctx, dtype, seqs, dim):
+    lens = [(0, 1, 63, 64, 65, 300, 511, 900)[b % 8] for b in range(seqs)]
+    if seqs == 1:
+        lens = [700]
+    c = Case(dtype, [1 + b % 2 for b in range(seqs)], [max(n, 0) for n in lens], 2, 5, dim, 16, device="cuda", behind=2, seed=seqs)
+    out = torch.full_like(c.q, 5.0).cuda()
+    c.check(c.attend(ctx, out=out))
+    assert (out[c.starts[-1]:] == 5).all()
+    ctx.sync_check()
+
+
 def test_many_short_sequences(ctx):
     c = Case(BF16, [1] * 700, [1 + b % 37 for b in range(700)], 4, 2, 64, 16, device="cuda", starts=False)
     c.check(c.attend(ctx))
