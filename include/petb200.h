@@ -235,7 +235,7 @@ typedef struct {
  * j + rotary / 2, or 2 j and 2 j + 1 where `interleaved`) is turned by the angle (pos0 + p) * inv_freq[j], formed in 64 bits.
  * inv_freq NULL or rotary 0: nothing is turned.  Sources are of type src_dtype (the cache's, or PETB200_F32), rounded once to the cache's;
  * q_out is of the cache's type.  q NULL: keys and values alone.  Rows outside all sequences, and tokens with p < 0, write nothing to
- * the cache; rows outside all sequences leave q_out as it was.  A page that two sequences of the call both append to is left undefined. */
+ * the cache; rows outside all sequences leave q_out as it was.  A page that two sequences of the call both append to is left undefined; q_out must not overlap a source. */
 int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const petb200_kv_rows *k,
                           const petb200_kv_rows *v, const petb200_kv_rows *q, const petb200_kv_rows *q_out, int q_heads, int src_dtype,
                           const float *inv_freq, int rotary, int interleaved, int pos0, petb200_stream stream);

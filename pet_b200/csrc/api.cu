@@ -28,12 +28,13 @@ extern "C" int petb200_ctx_create(int device, petb200_ctx **out) {
     }
     auto *ctx = new petb200_ctx();
     ctx->device = device;
-    cudaDeviceProp prop;
-    cudaGetDeviceProperties(&prop, device);
-    ctx->sm_count = prop.multiProcessorCount;
-    ctx->cc_major = prop.major;
-    ctx->cc_minor = prop.minor;
-    ctx->smem_optin = prop.sharedMemPerBlockOptin;
+    // (single attributes: all of a device's properties take milliseconds to gather)
+    int smem_optin = 0;
+    cudaDeviceGetAttribute(&ctx->sm_count, cudaDevAttrMultiProcessorCount, device);
+    cudaDeviceGetAttribute(&ctx->cc_major, cudaDevAttrComputeCapabilityMajor, device);
+    cudaDeviceGetAttribute(&ctx->cc_minor, cudaDevAttrComputeCapabilityMinor, device);
+    cudaDeviceGetAttribute(&smem_optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, device);
+    ctx->smem_optin = (size_t)smem_optin;
     if (cudaMalloc(&ctx->d_status, sizeof(int)) != cudaSuccess) {
         g_create_error = "ctx_create: status word allocation failed";
         delete ctx;

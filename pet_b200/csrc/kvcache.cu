@@ -64,11 +64,17 @@ template <typename S, typename T> __global__ void __launch_bounds__(kAppendThrea
     if (warp < ntok) {
         const int t = tok0 + warp;
         int b;
-        if (a.s.q_starts) { // the last sequence that begins at or before t: as many as do, all looked at together
-            int n = 0;
-            for (int i = lane; i <= a.s.seqs; i += 32)
-                n += __ldg(a.s.q_starts + i) <= t;
-            b = (int)__reduce_add_sync(0xffffffffu, n) - 1;
+        if (a.s.q_starts) { // the last sequence that begins at or before t: as many as do, up to 1024 of them looked at together
+            int from = 0, most = a.s.seqs + 1, n = 0;
+            while (most > 1024) { // (32 probes narrow down where more are)
+                const int step = ceil_div(most, 32), i = from + lane * step;
+                const int c = __popc(__ballot_sync(0xffffffffu, lane * step < most && __ldg(a.s.q_starts + i) <= t));
+                const int skip = max(c - 1, 0) * step;
+                from += skip, most = min(step, most - skip);
+            }
+            for (int i = lane; i < most; i += 32)
+                n += __ldg(a.s.q_starts + from + i) <= t;
+            b = from + (int)__reduce_add_sync(0xffffffffu, n) - 1;
         } else
             b = t / a.s.q_len;
         if (lane == 0) {
@@ -243,8 +249,8 @@ int check_cache(petb200_ctx *ctx, const char *what, const petb200_kv_cache *cach
     if (s->seqs && s->tokens) {
         if ((s->table_width && !s->page_table) || !s->kv_lens)
             return fail(ctx, PETB200_ERR_INVALID, "%s: no page table or no lengths", what);
-        if (c->pages && (!c->k || !c->v))
-            return fail(ctx, PETB200_ERR_INVALID, "%s: no cache", what);
+        if (!c->pages || !c->k || !c->v)
+            return fail(ctx, PETB200_ERR_INVALID, "%s: a cache without pages", what);
         if (!s->q_starts && s->tokens % s->seqs)
             return fail(ctx, PETB200_ERR_INVALID, "%s: %d tokens are not the same number for each of %d sequences", what, s->tokens, s->seqs);
     }

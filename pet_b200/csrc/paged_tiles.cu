@@ -160,11 +160,17 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
     const int split = blockIdx.x % splits, place = blockIdx.x / splits;
     if (warp == 0) { // units are laid end to end and taken from the last one down: later rows of a prompt see more keys
         const int seqs = one ? 1 : a.s.seqs;
-        auto count = [&](int b0) { return b0 + lane < seqs ? (unsigned)units_of(b0 + lane) : 0u; };
-        unsigned c = count(0), total = __reduce_add_sync(0xffffffffu, c);
+        auto count = [&](int b0) { return !one && a.s.q_starts && b0 + lane < seqs ? (unsigned)units_of(b0 + lane) : 0u; };
+        unsigned c = count(0), total = c;
+#pragma unroll 4
         for (int b0 = 32; b0 < seqs; b0 += 32)
-            total += __reduce_add_sync(0xffffffffu, count(b0));
-        if ((unsigned)place < total) {
+            total += count(b0);
+        total = __reduce_add_sync(0xffffffffu, total);
+        if (one || !a.s.q_starts) { // as many of each
+            const unsigned per = (unsigned)units_of(0), all = per * (unsigned)seqs;
+            if ((unsigned)place < all)
+                ctl.b = (int)((all - 1 - place) / per), ctl.unit = (int)((all - 1 - place) % per);
+        } else if ((unsigned)place < total) {
             const unsigned mine = total - 1 - place;
             unsigned run = 0;
             for (int b0 = 0; b0 < seqs && run <= mine; b0 += 32) {

@@ -69,6 +69,18 @@ def test_append_of_more_than_a_block_takes_and_without_queries(ctx):
     append_case(ctx, BF16, F32, [1200], [1200], 1, 40, 64, 32, 32, True)
 
 
+def test_many_sequences_of_uneven_prompts(ctx):
+    """More sequences than are looked at together: rows find theirs, with empty ones among them."""
+    new = [(3, 0, 1, 2)[b % 4] for b in range(2600)]
+    append_case(ctx, BF16, BF16, new, [n + b % 3 for b, n in enumerate(new)], 1, 1, 8, 4, 4, False)
+    new = [(17, 33, 0, 20)[b % 4] for b in range(150)]
+    c = Case(BF16, new, [n + b % 50 for b, n in enumerate(new)], 1, 4, 64, 16, device="cuda")
+    c.check(c.attend(ctx))
+    c = Case(F16, [20] * 70, [20 + b for b in range(70)], 2, 4, 64, 16, device="cuda", starts=False)
+    c.check(c.attend(ctx))
+    ctx.sync_check()
+
+
 def test_append_at_far_positions(ctx):
     """Angles of positions past 2^24: an fp32 product of position and frequency would be off by whole radians."""
     append_case(ctx, F32, F32, [3, 1], [5, 1], 1, 2, 64, 16, 32, False, pos0=2 ** 31 - 100)
@@ -420,6 +432,8 @@ def test_refused_by_the_library(ctx):
     refused(ERR_UNSUPPORTED, lambda: ctx.attention_paged(q, k, v, t, n, out=torch.zeros(2, 4, 65, device="cuda", dtype=BF16)[:, :, :64]))
     refused(ERR_UNSUPPORTED, lambda: ctx.kv_append(q[:, :2], q[:, 2:], odd, odd, t, n))
     refused(ERR_INVALID, lambda: ctx.kv_append(q[:, :2], q[:, 2:], k, v, t, n, inv_freq=torch.ones(33, device="cuda")))
+    refused(ERR_INVALID, lambda: ctx.kv_append(q[:, :2], q[:, 2:], k, v, t, n, q=q, q_out=q))
+    refused(ERR_INVALID, lambda: ctx.attention_paged(q, k[:0], v[:0], t, n))
     ctx.sync_check()
     for empty in (q[:0],):
         assert ctx.attention_paged(empty, k, v, t[:0], n[:0]).shape == (0, 4, 64)
