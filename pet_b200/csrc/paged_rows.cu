@@ -23,6 +23,7 @@
 #include "tc_ptx.cuh"
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace petb200 {
 namespace {
@@ -363,6 +364,118 @@ template <typename T, int DP> struct RowTile {
     }
 };
 
+// The same for up to RR rows in fp32 by multiply-adds: a tensor-core tile would be mostly empty, and splitting K and V in two for it is
+// what it spends its time on (one row of width 64: 420 instructions per 8 keys, 105 here).  LPK lanes share a key, four values of it
+// each; with width 64 the warp has two keys at a time.  Products and sums are plain fp32.
+template <int DP, int RR> struct FewRows {
+    using C = RowCfg<float, DP>;
+    static constexpr int LPK = DP / 4, KPP = 32 / LPK, NP = C::CK / KPP, QR = RR * 4;
+
+    float4 o[RR];
+    float m[RR], l[RR];
+
+    __device__ __forceinline__ static void load_q(const PagedArgs &a, const Unit &u, uint32_t (&qf)[QR]) {
+        const int d = (int)(threadIdx.x % LPK) * 4;
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+            const int row = u.rt * kRows + r, tok = row / a.group, hd = row - tok * a.group;
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (tok < u.ql && d < a.dim)
+                x = __ldg(reinterpret_cast<const uint4 *>((const float *)a.q + (long long)(u.t0 + tok) * a.q_tok + (long long)(u.h * a.group + hd) * a.q_head + d));
+            qf[4 * r] = x.x, qf[4 * r + 1] = x.y, qf[4 * r + 2] = x.z, qf[4 * r + 3] = x.w;
+        }
+    }
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int r = 0; r < RR; ++r)
+            o[r] = make_float4(0.f, 0.f, 0.f, 0.f), m[r] = -INFINITY, l[r] = 0.f;
+    }
+    // Keys [base, base + CK) of a stage; row r sees keys below lim[r].
+    __device__ __forceinline__ void step(const PagedArgs &a, const uint32_t (&qf)[QR], const unsigned char *stage, int base, const int (&lim)[RR], bool masked) {
+        const int lane = threadIdx.x & 31, piece = lane % LPK, mine = lane / LPK;
+        auto at = [&](int p) {
+            const int row = p * KPP + mine;
+            return row * (DP * 4) + RowTile<float, DP>::swz(row, piece) * 16;
+        };
+        float s[RR][NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const float4 k = *reinterpret_cast<const float4 *>(stage + at(p));
+#pragma unroll
+            for (int r = 0; r < RR; ++r) {
+                float x = __uint_as_float(qf[4 * r]) * k.x;
+                x = fmaf(__uint_as_float(qf[4 * r + 1]), k.y, x);
+                x = fmaf(__uint_as_float(qf[4 * r + 2]), k.z, x);
+                s[r][p] = fmaf(__uint_as_float(qf[4 * r + 3]), k.w, x);
+            }
+        }
+#pragma unroll
+        for (int w = LPK / 2; w > 0; w >>= 1)
+#pragma unroll
+            for (int r = 0; r < RR; ++r)
+#pragma unroll
+                for (int p = 0; p < NP; ++p)
+                    s[r][p] += __shfl_xor_sync(0xffffffffu, s[r][p], w);
+        bool grows = false;
+        float top[RR];
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+            top[r] = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                s[r][p] *= a.sl2;
+                if (masked)
+                    s[r][p] = base + p * KPP + mine < lim[r] ? s[r][p] : -INFINITY;
+                top[r] = fmaxf(top[r], s[r][p]);
+            }
+            if (KPP > 1)
+                top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], LPK & 31));
+            grows |= top[r] > m[r];
+        }
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int r = 0; r < RR; ++r) {
+                const float to = fmaxf(m[r], top[r]), f = m[r] == to ? 1.f : exp2_approx(m[r] - to);
+                m[r] = to, l[r] *= f;
+                o[r].x *= f, o[r].y *= f, o[r].z *= f, o[r].w *= f;
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+            const float z = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                s[r][p] = exp2_approx(s[r][p] - z);
+                l[r] += s[r][p];
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const float4 v = *reinterpret_cast<const float4 *>(stage + C::HALF + at(p));
+#pragma unroll
+            for (int r = 0; r < RR; ++r)
+                if (!masked || base + p * KPP + mine < lim[r]) // (0 times what a masked key holds could be NaN)
+                    o[r].x = fmaf(s[r][p], v.x, o[r].x), o[r].y = fmaf(s[r][p], v.y, o[r].y), o[r].z = fmaf(s[r][p], v.z, o[r].z), o[r].w = fmaf(s[r][p], v.w, o[r].w);
+        }
+    }
+    // The warp's sums where the block's warps meet; `seen[r]`: the row sees some of the warp's keys.
+    __device__ __forceinline__ void leave(float *wo, float2 *wm, const bool (&seen)[RR]) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int r = 0; r < RR; ++r) {
+            if (KPP > 1) {
+                o[r].x += __shfl_xor_sync(0xffffffffu, o[r].x, LPK & 31), o[r].y += __shfl_xor_sync(0xffffffffu, o[r].y, LPK & 31);
+                o[r].z += __shfl_xor_sync(0xffffffffu, o[r].z, LPK & 31), o[r].w += __shfl_xor_sync(0xffffffffu, o[r].w, LPK & 31);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], LPK & 31);
+            }
+            if (lane < LPK)
+                *reinterpret_cast<float4 *>(wo + r * C::MP + lane * 4) = o[r];
+            if (lane == 0)
+                wm[r] = make_float2(seen[r] ? fmaxf(m[r], -FLT_MAX) : -INFINITY, l[r]);
+        }
+    }
+};
+
 // {m, l, O} of one row from several places, in the order of the pieces.
 struct Joined {
     float M = -INFINITY, L = 0.f;
@@ -386,10 +499,12 @@ __device__ __forceinline__ void fma4(float4 &x, float w, float4 y) {
     x.x = fmaf(w, y.x, x.x), x.y = fmaf(w, y.y, x.y), x.z = fmaf(w, y.z, x.z), x.w = fmaf(w, y.w, x.w);
 }
 
-template <typename T, int DP>
+// FEW > 0 (fp32): no tile has more than that many rows.
+template <typename T, int DP, int FEW>
 __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int own_mode, int prefix_blocks, int prefix_pieces, int cluster) {
     using C = RowCfg<T, DP>;
-    using Tile = RowTile<T, DP>;
+    using Loader = RowTile<T, DP>;
+    using Tile = typename std::conditional<FEW == 0, RowTile<T, DP>, FewRows<DP, FEW ? FEW : 1>>::type;
     pdl_prologue();
     extern __shared__ __align__(1024) unsigned char smem[];
     __shared__ unsigned tmp[kRowWarps];
@@ -478,6 +593,10 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
         const int r0 = u.rt * kRows + g, tok0 = r0 / a.group, tok1 = (r0 + 8) / a.group;
         const int lim0 = tok0 < u.ql ? visible(tok0, u.ql, u.own) : 0, lim1 = tok1 < u.ql ? visible(tok1, u.ql, u.own) : 0;
         const int full = visible(u.rt * kRows / a.group, u.ql, u.own); // keys that every row sees
+        [[maybe_unused]] auto few_lim = [&](int r) {
+            const int tok = (u.rt * kRows + r) / a.group;
+            return tok < u.ql ? visible(tok, u.ql, u.own) : 0;
+        };
 
         Tile tile;
         tile.reset();
@@ -486,7 +605,7 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
         for (int st = 0; st < C::NST - 1; ++st) {
             const int key = (s0 + st) * C::KT + base0;
             if (s0 + st < s1 && key < u.n)
-                Tile::fetch(a, u, ring + st * 2 * C::HALF, key, u.n);
+                Loader::fetch(a, u, ring + st * 2 * C::HALF, key, u.n);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
         uint32_t qf[Tile::QR];
@@ -499,12 +618,19 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
             {
                 const int nx = i + C::NST - 1, key = nx * C::KT + base0, to = st == 0 ? C::NST - 1 : st - 1;
                 if (nx < s1 && key < u.n)
-                    Tile::fetch(a, u, ring + to * 2 * C::HALF, key, u.n);
+                    Loader::fetch(a, u, ring + to * 2 * C::HALF, key, u.n);
                 asm volatile("cp.async.commit_group;" ::: "memory");
             }
             const int key = i * C::KT + base0;
             if (key < u.n)
-                tile.step(a, qf, ring + st * 2 * C::HALF, ring_p + st * 2 * C::HALF, key, lim0, lim1, key + C::CK > full);
+                if constexpr (FEW > 0) {
+                    int lim[FEW];
+#pragma unroll
+                    for (int r = 0; r < FEW; ++r)
+                        lim[r] = few_lim(r);
+                    tile.step(a, qf, ring_p + st * 2 * C::HALF, key, lim, key + C::CK > full);
+                } else
+                    tile.step(a, qf, ring + st * 2 * C::HALF, ring_p + st * 2 * C::HALF, key, lim0, lim1, key + C::CK > full);
             st = st == C::NST - 1 ? 0 : st + 1;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -513,28 +639,36 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
         // ---- the warps meet: {m, l} and O of each in its own stages --------------------------------------------------
         float *wo = reinterpret_cast<float *>(ring_p);
         float2 *wm = reinterpret_cast<float2 *>(wo + kRows * C::MP);
+        if constexpr (FEW > 0) {
+            bool seen[FEW];
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            float l = tile.l[r];
-            l += __shfl_xor_sync(0xffffffffu, l, 1);
-            l += __shfl_xor_sync(0xffffffffu, l, 2);
-            const int lim = r ? lim1 : lim0, seen = lim > s0 * C::KT + base0 && s1 > s0; // this warp's first key at least
-            if ((lane & 3) == 0)
-                wm[g + 8 * r] = make_float2(seen ? fmaxf(tile.m[r], -FLT_MAX) : -INFINITY, l);
-        }
-        if constexpr (C::f32) {
-#pragma unroll
-            for (int t = 0; t < DP / 8; t += 4)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    *reinterpret_cast<float4 *>(&wo[(g + 8 * (e >> 1)) * C::MP + Tile::column(t, e)]) =
-                        make_float4(tile.o[t][e], tile.o[t + 1][e], tile.o[t + 2][e], tile.o[t + 3][e]);
+            for (int r = 0; r < FEW; ++r)
+                seen[r] = few_lim(r) > s0 * C::KT + base0 && s1 > s0; // this warp's first key at least
+            tile.leave(wo, wm, seen);
         } else {
 #pragma unroll
-            for (int t = 0; t < DP / 8; ++t)
+            for (int r = 0; r < 2; ++r) {
+                float l = tile.l[r];
+                l += __shfl_xor_sync(0xffffffffu, l, 1);
+                l += __shfl_xor_sync(0xffffffffu, l, 2);
+                const int lim = r ? lim1 : lim0, seen = lim > s0 * C::KT + base0 && s1 > s0; // this warp's first key at least
+                if ((lane & 3) == 0)
+                    wm[g + 8 * r] = make_float2(seen ? fmaxf(tile.m[r], -FLT_MAX) : -INFINITY, l);
+            }
+            if constexpr (C::f32) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r)
-                    *reinterpret_cast<float2 *>(&wo[(g + 8 * r) * C::MP + Tile::column(t, 0)]) = make_float2(tile.o[t][2 * r], tile.o[t][2 * r + 1]);
+                for (int t = 0; t < DP / 8; t += 4)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        *reinterpret_cast<float4 *>(&wo[(g + 8 * (e >> 1)) * C::MP + Tile::column(t, e)]) =
+                            make_float4(tile.o[t][e], tile.o[t + 1][e], tile.o[t + 2][e], tile.o[t + 3][e]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < DP / 8; ++t)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        *reinterpret_cast<float2 *>(&wo[(g + 8 * r) * C::MP + Tile::column(t, 0)]) = make_float2(tile.o[t][2 * r], tile.o[t][2 * r + 1]);
+            }
         }
         __syncthreads();
         {
@@ -724,8 +858,8 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) k_paged_joi
         store4<T>((T *)a.out + (long long)tok * a.o_tok + (long long)head * a.o_head + col, settle(v, M, L));
 }
 
-template <typename T, int DP>
-int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int n_prefix, cudaStream_t s) {
+template <typename T, int DP, int FEW>
+int rows_launch_as(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int n_prefix, cudaStream_t s) {
     using C = RowCfg<T, DP>;
     const long long rows = (long long)a.s.tokens * a.group;
     // Row tiles there can be: a sequence's last one may be short.
@@ -756,7 +890,7 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
         return PETB200_OK;
     if (bytes > ws_bytes)
         return fail(ctx, PETB200_ERR_INVALID, "attention over pages: a workspace of %zu bytes, %zu are needed", ws_bytes, bytes);
-    if (int rc = raise_smem(ctx, (const void *)k_paged_rows<T, DP>, C::SMEM))
+    if (int rc = raise_smem(ctx, (const void *)k_paged_rows<T, DP, FEW>, C::SMEM))
         return rc;
     if (mode == kModeCluster) {
         cudaLaunchConfig_t cfg{};
@@ -767,10 +901,10 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
-        (void)cudaLaunchKernelEx(&cfg, k_paged_rows<T, DP>, a, mode, 0, 1, cluster);
+        (void)cudaLaunchKernelEx(&cfg, k_paged_rows<T, DP, FEW>, a, mode, 0, 1, cluster);
         return launched(ctx, "k_paged_rows");
     }
-    launch_pdl(k_paged_rows<T, DP>, dim3(grid + (unsigned)prefix_blocks), kRowThreads, C::SMEM, s, a, mode, (int)prefix_blocks, std::max(1, n_prefix), 1);
+    launch_pdl(k_paged_rows<T, DP, FEW>, dim3(grid + (unsigned)prefix_blocks), kRowThreads, C::SMEM, s, a, mode, (int)prefix_blocks, std::max(1, n_prefix), 1);
     int rc = launched(ctx, "k_paged_rows");
     if (rc || mode != kModeRanges)
         return rc;
@@ -778,6 +912,18 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
     const int four = (int)std::min<long long>(kRows / 4, a.s.q_starts ? kRows / 4 : ((long long)a.s.q_len * a.group + 3) / 4);
     launch_pdl(k_paged_join<T, DP>, dim3(grid, (unsigned)four), 256, 0, s, a);
     return launched(ctx, "k_paged_join");
+}
+
+template <typename T, int DP>
+int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int n_prefix, cudaStream_t s) {
+    if constexpr (sizeof(T) == 4) { // (the prefix's tiles have other sequences' rows in them)
+        const long long rows = a.s.q_starts || n_prefix ? kRows : (long long)a.s.q_len * a.group;
+        if (rows == 1)
+            return rows_launch_as<T, DP, 1>(ctx, a, ws, ws_bytes, need, n_prefix, s);
+        if (rows <= 4)
+            return rows_launch_as<T, DP, 4>(ctx, a, ws, ws_bytes, need, n_prefix, s);
+    }
+    return rows_launch_as<T, DP, 0>(ctx, a, ws, ws_bytes, need, n_prefix, s);
 }
 
 template <typename T, int DP> int join_launch(petb200_ctx *ctx, const PagedArgs &a, cudaStream_t s) {

@@ -155,6 +155,27 @@ def test_masked_keys_never_contribute(ctx, dtype, new, bad):
     assert ((got[:-1] - want[:-1]).abs() <= tol[:-1]).all() and torch.isnan(got[-1]).all()
 
 
+@pytest.mark.parametrize("new,group", [(1, 1), (4, 1), (2, 2), (1, 3)])
+@pytest.mark.parametrize("dim", [8, 64, 104, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_few_rows_in_full_precision(ctx, new, group, dim, bad):
+    """Up to four rows of fp32: lengths around a warp's and a block's step, and newest keys that hold no numbers."""
+    c = Case(F32, [new] * 9, [max(n, new) for n in (1, 7, 8, 9, 31, 33, 130, 700, 2050)], 2, group, dim, 16, device="cuda", starts=False)
+    c.check(c.attend(ctx))
+    if new > 1:
+        want, tol = c.want()
+        for b in range(9):
+            at = c.lens[b] - 1
+            c.v[c.table[b, at // c.page].long(), at % c.page, 1, 3] = bad
+            c.k[c.table[b, at // c.page].long(), at % c.page, 0, 2] = bad
+        got = c.attend(ctx).double().cpu()
+        for b in range(9):
+            rows, last = slice(c.starts[b], c.starts[b + 1] - 1), c.starts[b + 1] - 1
+            assert ((got[rows] - want[rows]).abs() <= tol[rows]).all()
+            assert not torch.isfinite(got[last, group:, 3]).any() and (torch.isnan(got[last, :group]).all() or bad == math.inf)
+    ctx.sync_check()
+
+
 @pytest.mark.parametrize("dtype", ALL)
 def test_long_sequences_among_short_ones(ctx, dtype):
     """Ranges of work that cut a sequence many times, and take many sequences whole."""
