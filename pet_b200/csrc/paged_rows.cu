@@ -11,8 +11,10 @@
 //
 // Work is split by ranges: the key steps of all (sequence, row tile, key head) units are laid end to end and every CTA takes an
 // equal share, whatever the lengths; a unit that crosses a border leaves one piece per CTA, and k_paged_join adds the pieces in order.
+// Few units of moderate length go to a thread-block cluster each instead, which adds its sums through shared memory; many units, or
+// units of a few steps, to a CTA each.  64 sequences of up to 8000 keys (1.05 GB): 182 us, 5.8 TB/s; one token on 1500 keys: 11 us a call.
 //
-// fp32 runs on the TF32 tensor cores with both operands split in two (x = hi + lo, hi the upper 11 bits: hi hi + hi lo + lo hi,
+// fp32 runs on the TF32 tensor cores (up to four rows: on multiply-adds, see FewRows) with both operands split in two (x = hi + lo, hi the upper 11 bits: hi hi + hi lo + lo hi,
 // 2^-21 of a product left out), and the product with V starts from zero for every 8 keys and is added in registers, since a tensor core's
 // own accumulation cuts off instead of rounding.  Scores, statistics and sums are fp32 for every type; probabilities are
 // rounded to the cache's type for the second product (16-bit types; the sum of the row takes them unrounded).

@@ -5,10 +5,17 @@
 //
 // A unit is 256 rows = (token, query head) pairs that share one key head, as two tiles of 128, against 128 keys at a time.  TMEM holds
 // both tiles' scores (fp32) and outputs, all 512 columns at head width 128; P takes its scores' place as 16-bit values and is the A operand
-// of the second product from there.  Roles: warps 0-3 and 4-7 do the softmax of a tile each (a thread owns a row), warps 8-11 fetch,
-// warp 12 issues the products.  The products of one tile run under the softmax of the other.
+// of the second product from there.  Roles: warps 0-3 and 4-7 do the softmax of a tile each (a thread owns a row), warps 8-11 fetch
+// (warp 10 the keys, the others first the queries), warp 15 issues the products.  The products of one tile run under the softmax of
+// the other.
 //   tensor pipe  2 x (S: 128 x 128 x D, O: 128 x D x 128) = 2048 cycles per 128 keys at D = 128
 //   exponentials 2 x 16384 at 16 a cycle                  = 2048 cycles
+// Measured at D = 128: 3360 cycles per 128 keys.  What bounds it is the chain of one tile: its softmax (1800 cycles: 330 for reading the
+// scores, 220 for the maximum, 1250 for the powers, whose 450 instructions come at three cycles each), the hand-over (350) and its
+// two products (1270).  Tried and no faster: part of the powers as polynomials on the FMA pipe (more instructions), two threads a row,
+// quarters of a tile in a rolled loop, the maximum of the tile before taken first and checked beside the powers, and blocks that
+// stay and take unit after unit (registers spilled).  Beside the keys a unit costs 11 k cycles until its first scores and 5 k for its
+// results.  500 tokens x 8 heads on 33 k keys: 154 us, 870 TFLOP/s; tensor pipe busy 58 % (profiles/paged_attention.md).
 // The maximum moves only where a row's grows by more than 2^8 over the one in use (then O and l are scaled, by the softmax warps): the
 // sums stay within range and any m gives the same quotient.
 //

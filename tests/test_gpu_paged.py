@@ -363,6 +363,38 @@ def test_captured_call_reads_new_lengths(ctx):
     c.check(out)
 
 
+def test_captured_layer_with_a_prefix(ctx):
+    """Append, attention behind a prefix and attention of prompts in one graph, replayed on other inputs and lengths."""
+    heads, dim, page, prefix = 2, 64, 16, 100
+    g = torch.Generator().manual_seed(9)
+    kc, vc = (torch.randn(60, page, heads, dim, generator=g).to(BF16).cuda() for _ in "kv")
+    table = torch.arange(60, dtype=torch.int32)[10:58].view(3, 16).contiguous().cuda()
+    head = torch.arange(7, dtype=torch.int32).cuda()
+    freq = (10000.0 ** (-torch.arange(32) / 32)).cuda()
+    lens = torch.tensor([4, 9, 1], dtype=torch.int32, device="cuda")
+    long, starts = torch.tensor([70, 90, 80], dtype=torch.int32, device="cuda"), torch.tensor([0, 70, 130, 200], dtype=torch.int32, device="cuda")
+    x, p = torch.zeros(3, 8, dim, device="cuda", dtype=BF16), torch.zeros(200, 4, dim, device="cuda", dtype=BF16)
+
+    def layer():
+        q = ctx.kv_append(x[:, 4:6], x[:, 6:], kc, vc, table, lens, q=x[:, :4], inv_freq=freq, pos0=prefix)
+        return q, ctx.attention_prefix(q, kc, vc, head, prefix, table, lens), ctx.attention_paged(p, kc, vc, table, long, q_starts=starts)
+    layer()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layer()
+    x.copy_(torch.randn(3, 8, dim, generator=g).to(BF16))
+    p.copy_(torch.randn(200, 4, dim, generator=g).to(BF16))
+    lens.copy_(torch.tensor([40, 1, 200], dtype=torch.int32))
+    long.copy_(torch.tensor([200, 60, 70], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    replayed = [t.clone() for t in got]
+    assert all(torch.equal(a, b) for a, b in zip(replayed, layer()))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(replayed, got))
+
+
 def test_calls_on_two_streams(ctx):
     """Workspaces are a call's own: calls that overlap give what they give alone."""
     cases = [Case(F16, [1] * 8, [700 + 31 * b for b in range(8)], 2, 4, 128, device="cuda", starts=False, seed=s, prefix=p) for s, p in ((1, 0), (2, 300))]
