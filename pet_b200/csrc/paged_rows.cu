@@ -860,6 +860,43 @@ template <typename T, int DP> __global__ void __launch_bounds__(256) k_paged_joi
         store4<T>((T *)a.out + (long long)tok * a.o_tok + (long long)head * a.o_head + col, settle(v, M, L));
 }
 
+// The same for up to four pieces: a warp per row, all that it reads in one trip, and registers for eight blocks an SM instead of two
+// (11 k rows of two pieces: 19 us with the pairs of warps above).
+template <typename T, int DP> __global__ void __launch_bounds__(256) k_paged_join_four(const PagedArgs a) {
+    pdl_prologue();
+    const int lane = threadIdx.x & 31, heads = a.hkv * a.group, col = DP == 128 ? lane * 4 : (lane & 15) * 4;
+    const long long rows = (long long)a.s.tokens * a.group, id = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (id >= rows * a.hkv)
+        return;
+    const int tok = (int)(id / heads), head = (int)(id - (long long)tok * heads), h = head / a.group;
+    const int first = a.s.q_starts ? __ldg(a.s.q_starts) : 0, last = a.s.q_starts ? __ldg(a.s.q_starts + a.s.seqs) : a.s.tokens;
+    float2 ml[4];
+    float4 x[4];
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        ml[p] = make_float2(-INFINITY, 0.f);
+        x[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (p < a.pieces) {
+            const long long at = ((long long)p * a.hkv + h) * rows + (long long)tok * a.group + (head - h * a.group);
+            ml[p] = a.pml[at];
+            x[p] = *reinterpret_cast<const float4 *>(a.po + at * DP + col);
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+        M = fmaxf(M, ml[p].x);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+        const float f = piece_weight(ml[p].x, M);
+        L = fmaf(f, ml[p].y, L);
+        fma4(v, f, x[p]);
+    }
+    if (tok >= first && tok < last && lane * 4 < a.dim) // (rows outside all sequences stay as they were)
+        store4<T>((T *)a.out + (long long)tok * a.o_tok + (long long)head * a.o_head + col, settle(v, M, L));
+}
+
 template <typename T, int DP, int FEW>
 int rows_launch_as(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t *need, int n_prefix, cudaStream_t s) {
     using C = RowCfg<T, DP>;
@@ -930,7 +967,10 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
 
 template <typename T, int DP> int join_launch(petb200_ctx *ctx, const PagedArgs &a, cudaStream_t s) {
     const long long rows = (long long)a.s.tokens * a.group * a.hkv;
-    launch_pdl(k_paged_join_rows<T, DP>, dim3((unsigned)((rows + 3) / 4)), 256, 0, s, a);
+    if (a.pieces <= 4)
+        launch_pdl(k_paged_join_four<T, DP>, dim3((unsigned)((rows + 7) / 8)), 256, 0, s, a);
+    else
+        launch_pdl(k_paged_join_rows<T, DP>, dim3((unsigned)((rows + 3) / 4)), 256, 0, s, a);
     return launched(ctx, "k_paged_join_rows");
 }
 

@@ -10,8 +10,8 @@
 // the other.
 //   tensor pipe  2 x (S: 128 x 128 x D, O: 128 x D x 128) = 2048 cycles per 128 keys at D = 128
 //   exponentials 2 x 16384 at 16 a cycle                  = 2048 cycles
-// Measured at D = 128: 3360 cycles per 128 keys.  What bounds it is the chain of one tile: its softmax (1800 cycles: 330 for reading the
-// scores, 220 for the maximum, 1250 for the powers, whose 450 instructions come at three cycles each), the hand-over (350) and its
+// Measured at D = 128: 3360 cycles per 128 keys.  What bounds it is the chain of one tile: its softmax (1800 cycles: 220 for reading the
+// scores, 320 for the maximum, 1280 for the powers, whose 450 instructions come at three cycles each), the hand-over (350) and its
 // two products (1270).  Tried and no faster: part of the powers as polynomials on the FMA pipe (more instructions), two threads a row,
 // quarters of a tile in a rolled loop, the maximum of the tile before taken first and checked beside the powers, and blocks that
 // stay and take unit after unit (registers spilled).  Beside the keys a unit costs 11 k cycles until its first scores and 5 k for its
