@@ -909,11 +909,12 @@ int rows_launch_as(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, siz
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "attention over pages: %lld row tiles of up to %lld keys are more than one call takes", units, keys);
     const int slots = ctx->sm_count * C::CTAS;
     // Units as they are where there are several rounds of them (ranges would cut each in two for a gain of a part of a round), or
-    // where a unit is a few steps (a second launch would cost more than they).
+    // where a unit is a few steps (a second launch would cost more than they).  Two rounds do where units are short: 1024 units of up to
+    // 500 keys behind a prefix 96 us for the call, 114 with ranges; units of thousands of keys lose 7 % that way.
     // Few units of moderate length go to a cluster of blocks each, which add their sums through shared memory: one launch and no
     // workspace (one token on 1500 keys, 8 units: 15.5 us a call with ranges, whose second launch alone costs the host 2.5).
     const int cluster = n_prefix || a.piece_out >= 0 || steps <= 4 ? 0 : units * 8 <= slots && steps <= 64 ? 8 : units * 4 <= slots && steps <= 32 ? 4 : 0;
-    const int mode = cluster ? kModeCluster : units >= 4ll * slots || steps <= 4 ? kModeUnits : kModeRanges;
+    const int mode = cluster ? kModeCluster : units >= (steps <= 16 ? 2ll : 4ll) * slots || steps <= 4 ? kModeUnits : kModeRanges;
     const unsigned grid = (unsigned)(mode == kModeRanges ? std::min<long long>(slots, units * steps) : mode == kModeCluster ? units * cluster : units);
     size_t bytes = 0;
     if (mode == kModeRanges) {
