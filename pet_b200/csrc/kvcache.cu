@@ -280,8 +280,15 @@ PagedArgs attention_args(petb200_ctx *ctx, const petb200_kv_cache *cache, const 
     return a;
 }
 
-// Rows of one sequence and key head from which a 128-row tile is used, be it part full.
-constexpr int kTileFrom = 64;
+// Rows of a sequence and key head from which a 128-row tile is used, be it part full: as soon as 16 rows are not enough, and its keys would
+// be read again.  16 sequences of 4000 keys, 8 key heads of 128, us with 16-row tiles / 128-row tiles: 16 rows 57 / 66, 32 rows 85 / 67,
+// 64 rows 147 / 68; 32 sequences of 700 keys: 33 / 36, 49 / 36, 67 / 36.
+constexpr int kTileFrom = 17;
+// Rows from which a sequence behind a shared prefix reads it by itself: a row for every 48 shared keys, at most 192.  Rows that go together
+// fill their tiles but meet their own keys in 16-row tiles; alone a sequence's tile is part empty for all of the prefix.  us together /
+// alone: 16 sequences behind 4000 keys, 40 own: 24 rows 37 / 65, 64 rows 57 / 66, 128 rows 74 / 67; 8 behind 16000: 128 rows 106 / 126; 32
+// behind 1000, 300 own: 24 rows 63 / 55, 64 rows 77 / 55.
+long long alone_from(int prefix_len) { return std::min(192, std::max(kTileFrom, prefix_len / 48)); }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -291,14 +298,15 @@ int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, in
     a.s.table0 = prefix_table;
     a.s.n0 = prefix_len;
     const bool halves = dtype != PETB200_F32;
-    const bool full = rows / a.s.seqs >= kTileFrom; // a sequence's rows by themselves are enough for the tensor cores' tiles
-    // Such a sequence gains nothing from the others: its keys, shared and own, are read as one run.
-    if (prefix_len == 0 || a.s.seqs == 1 || full)
-        return halves && full ? paged_tiles_run(ctx, dtype, a, ws, ws_bytes, need, 0, s) : paged_rows_run(ctx, dtype, a, ws, ws_bytes, need, 0, s);
+    const long long each = rows / a.s.seqs;
+    // A sequence with rows enough for tiles of its own gains nothing from the others: its keys, shared and own, are read as one run.
+    if (prefix_len == 0 || a.s.seqs == 1 || each >= alone_from(prefix_len))
+        return halves && each >= kTileFrom ? paged_tiles_run(ctx, dtype, a, ws, ws_bytes, need, 0, s) : paged_rows_run(ctx, dtype, a, ws, ws_bytes, need, 0, s);
     // All tokens as one sequence against the shared keys, in pieces; each sequence against its own, as one more piece; the pieces of a row added.
     PagedArgs p = a;
     p.s.kv_lens = nullptr, p.s.q_starts = nullptr;
-    const bool tiles = halves && rows >= kTileFrom;
+    // (16-row tiles share their launch with the own keys, and are done before a second launch: 32 rows against 1901 keys 16 us, 26 in tiles)
+    const bool tiles = halves && rows >= 64;
     int pieces;
     if (tiles)
         pieces = paged_tiles_pieces(ctx, p);

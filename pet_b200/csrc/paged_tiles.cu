@@ -15,7 +15,7 @@
 // two products (1270).  Tried and no faster: part of the powers as polynomials on the FMA pipe (more instructions), two threads a row,
 // quarters of a tile in a rolled loop, the maximum of the tile before taken first and checked beside the powers, and blocks that
 // stay and take unit after unit (registers spilled).  Beside the keys a unit costs 11 k cycles until its first scores and 5 k for its
-// results.  500 tokens x 8 heads on 33 k keys: 154 us, 870 TFLOP/s; tensor pipe busy 58 % (profiles/paged_attention.md).
+// results.  500 tokens x 16 heads on 33 k keys: 149 us, 900 TFLOP/s; tensor pipe busy 58 % (profiles/paged_attention.md).
 // The maximum moves only where a row's grows by more than 2^8 over the one in use (then O and l are scaled, by the softmax warps): the
 // sums stay within range and any m gives the same quotient.
 //
