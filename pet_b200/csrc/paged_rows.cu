@@ -20,7 +20,8 @@
 // rounded to the cache's type for the second product (16-bit types; the sum of the row takes them unrounded).
 //
 // Rows that see no key give zeros.  A masked key never contributes, whatever its value: its score is replaced before the
-// maximum, and non-finite values of its v are taken out of the stage before the product (see `scrub`).
+// maximum, and non-finite values of its v are taken out of the stage before the product (see `scrub`).  Infinities that are seen give what
+// the formula gives: a score of -inf weighs nothing, one of +inf makes the row NaN, an infinite v is its column's result.
 #include "paged.cuh"
 #include "tc_ptx.cuh"
 #include <algorithm>
@@ -70,11 +71,17 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x = hi + lo with hi the upper 11 bits of x; an infinity is all in hi.
+// x = hi + lo with hi the upper 11 bits of x.  lo is NaN where x is not finite, so that a step with such a value shows in its sums.
 __device__ __forceinline__ void split_tf32(uint32_t x, uint32_t &hi, uint32_t &lo) {
     hi = x & 0xffffe000u;
-    const float h = __uint_as_float(hi), f = __uint_as_float(x);
-    lo = h == f ? 0u : __float_as_uint(f - h);
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
+// The two parts where x may be infinite: `hi` has it in the product of the upper parts, `cross` (0 there) goes with the other operand's lo, which
+// may be 0.
+__device__ __forceinline__ void split_careful(uint32_t x, uint32_t &hi, uint32_t &lo, uint32_t &cross) {
+    split_tf32(x, hi, lo);
+    const bool inf = (x & 0x7fffffffu) == 0x7f800000u;
+    lo = inf ? 0u : lo, cross = inf ? 0u : hi;
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (std::is_same<T, __half>::value)
@@ -200,8 +207,9 @@ template <typename T, int DP> struct RowTile {
         return C::f32 ? (t >> 2) * 32 + 8 * c + 4 * (e & 1) + (t & 3) : t * 8 + 2 * c + (e & 1);
     }
 
-    // Non-finite values of v in a step whose keys some rows do not see: a product with probability 0 would be NaN.  They are
-    // added where they are seen (an infinity or a NaN outlives any factor) and taken out of the stage.
+    // Non-finite values of v in a step whose keys some rows do not see (a product with probability 0 would be NaN), in fp32 in any step (so
+    // would one with a lower part of 0).  They are added where they are seen (an infinity or a NaN outlives any factor) and taken out of
+    // the stage.
     __device__ __forceinline__ void scrub(unsigned char *vst, int base, int lim0, int lim1) {
         const int lane = threadIdx.x & 31;
         T *v = reinterpret_cast<T *>(vst);
@@ -226,40 +234,53 @@ template <typename T, int DP> struct RowTile {
         __syncwarp();
     }
 
+    // fp32: the scores of the stage's eight keys.  CAREFUL: right for infinite keys too.  (A query with an infinity is NaN either way: all its
+    // scores are infinite or NaN.)
+    template <bool CAREFUL> __device__ __forceinline__ static void scores_f32(const uint32_t (&qf)[QR], uint32_t stage, float (&s)[4]) {
+        const int lane = threadIdx.x & 31, row = lane & 7;
+        float x[3][4];
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                x[i][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) { // two k steps of 8 per ldmatrix: pieces 4 k .. 4 k + 3 of the 8 keys
+            uint32_t r[4];
+            ldsm4(stage + row * (DP * 4) + swz(row, 4 * k + (lane >> 3)) * 16, r);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t bh[2], bl[2], bx[2], qh[4], ql[4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (CAREFUL)
+                        split_careful(r[2 * h + e], bh[e], bl[e], bx[e]);
+                    else
+                        split_tf32(r[2 * h + e], bh[e], bl[e]), bx[e] = bh[e];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    qh[e] = qf[(2 * k + h) * 8 + e], ql[e] = qf[(2 * k + h) * 8 + 4 + e];
+                mma8(x[0], qh, bh[0], bh[1]);
+                mma8(x[1], qh, bl[0], bl[1]);
+                mma8(x[2], ql, bx[0], bx[1]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            s[e] = x[0][e] + (x[1][e] + x[2][e]);
+    }
+
     // One step: keys [base, base + CK) in `stage`; row g sees keys below lim0, row g + 8 below lim1.
     __device__ __forceinline__ void step(const PagedArgs &a, const uint32_t (&qf)[QR], uint32_t stage, unsigned char *stage_p, int base,
                                          int lim0, int lim1, bool masked) {
         const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
         float s[NJ][4];
         if constexpr (C::f32) {
-            float x[3][4];
-#pragma unroll
-            for (int i = 0; i < 3; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    x[i][e] = 0.f;
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) { // two k steps of 8 per ldmatrix: pieces 4 k .. 4 k + 3 of the 8 keys
-                uint32_t r[4];
-                const int row = lane & 7;
-                ldsm4(stage + row * (DP * 4) + swz(row, 4 * k + (lane >> 3)) * 16, r);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t bh[2], bl[2];
-                    split_tf32(r[2 * h], bh[0], bl[0]);
-                    split_tf32(r[2 * h + 1], bh[1], bl[1]);
-                    uint32_t qh[4], ql[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        qh[e] = qf[(2 * k + h) * 8 + e], ql[e] = qf[(2 * k + h) * 8 + 4 + e];
-                    mma8(x[0], qh, bh[0], bh[1]);
-                    mma8(x[1], qh, bl[0], bl[1]);
-                    mma8(x[2], ql, bh[0], bh[1]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                s[0][e] = x[0][e] + (x[1][e] + x[2][e]);
+            scores_f32<false>(qf, stage, s[0]);
+            // A value that is not finite makes its sums NaN through its lower part: such a step is done again with infinities kept out of the
+            // cross products, since 0 x infinity is not what the formula has there.
+            if (__any_sync(0xffffffffu, s[0][0] != s[0][0] || s[0][1] != s[0][1] || s[0][2] != s[0][2] || s[0][3] != s[0][3]))
+                scores_f32<true>(qf, stage, s[0]);
         } else {
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
@@ -311,7 +332,7 @@ template <typename T, int DP> struct RowTile {
                 s[j][e] = exp2_approx(s[j][e] - z0), s[j][e + 2] = exp2_approx(s[j][e + 2] - z1);
                 l[0] += s[j][e], l[1] += s[j][e + 2];
             }
-        if (masked) {
+        if (!C::f32 && masked) {
             bool bad = false;
             const uint4 *v = reinterpret_cast<const uint4 *>(stage_p + C::HALF);
             for (int i = lane; i < C::CK * C::CPR; i += 32) {
@@ -335,18 +356,30 @@ template <typename T, int DP> struct RowTile {
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) { // lane g's column of tile 4 i + e is 32 i + 4 g + e
                 const int r0 = 2 * c, r1 = 2 * c + 1;
-                const uint4 w0 = *reinterpret_cast<const uint4 *>(vst + r0 * (DP * 4) + swz(r0, 8 * i + g) * 16);
-                const uint4 w1 = *reinterpret_cast<const uint4 *>(vst + r1 * (DP * 4) + swz(r1, 8 * i + g) * 16);
-                const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+                uint32_t h0[4], l0[4], h1[4], l1[4];
+                auto load = [&]() { // answers whether all of it is finite
+                    const uint4 w0 = *reinterpret_cast<const uint4 *>(vst + r0 * (DP * 4) + swz(r0, 8 * i + g) * 16);
+                    const uint4 w1 = *reinterpret_cast<const uint4 *>(vst + r1 * (DP * 4) + swz(r1, 8 * i + g) * 16);
+                    const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        split_tf32(x0[e], h0[e], l0[e]);
+                        split_tf32(x1[e], h1[e], l1[e]);
+                        sum += __uint_as_float(l0[e]) + __uint_as_float(l1[e]);
+                    }
+                    return sum == sum;
+                };
+                if (__any_sync(0xffffffffu, !load())) { // (none of the columns before had such a value, and none behind has one any more)
+                    scrub(stage_p + C::HALF, base, lim0, lim1);
+                    load();
+                }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    uint32_t h0, l0, h1, l1;
-                    split_tf32(x0[e], h0, l0);
-                    split_tf32(x1[e], h1, l1);
                     float y[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma8(y, pl, h0, h1);
-                    mma8(y, ph, l0, l1);
-                    mma8(y, ph, h0, h1);
+                    mma8(y, pl, h0[e], h1[e]);
+                    mma8(y, ph, l0[e], l1[e]);
+                    mma8(y, ph, h0[e], h1[e]);
 #pragma unroll
                     for (int z = 0; z < 4; ++z)
                         o[4 * i + e][z] += y[z];
