@@ -40,7 +40,7 @@ constexpr int kTileRows = 128, kTileKeys = 128, kTileThreads = 512;
 constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(256 * (kSoftmaxRegs + kOtherRegs) <= kTileThreads * 128, "more registers than the block was launched with: setmaxnreg would wait forever");
 constexpr int kLag = 2; // stages whose copies a fetching thread leaves in flight before it reports the one before them
-constexpr float kGrowth = 8.f;
+constexpr float kGrowth = 8.f, kLargeScore = 1048576.f;
 
 template <int DP> struct TileCfg {
     static constexpr int STAGE = kTileKeys * DP * 2;
@@ -505,6 +505,17 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                     float top = ptx::max3_nan(ptx::max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * a.sl2;
                     if (!(top < INFINITY))
                         top = NAN; // the formula's inf - inf, or a score that is none: the row's result is NaN
+                    // Below, a score's product with the scale is not rounded, as m is: of a score t the difference is up to 2^-24 t, which would
+                    // be a power out of range where t is large.  Such scores are rounded first.
+                    float2 sl2 = make_float2(a.sl2, a.sl2);
+                    if (__any_sync(0xffffffffu, fabsf(top) >= kLargeScore && top > -INFINITY)) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                s[c][i] = __float_as_uint(__uint_as_float(s[c][i]) * a.sl2);
+                        sl2 = make_float2(1.f, 1.f);
+                    }
                     if (j == 0)
                         m = top;
                     else if (__any_sync(0xffffffffu, top - m > kGrowth || top != top)) {
@@ -524,7 +535,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                         }
                     }
                     const float z = m == -INFINITY ? 0.f : -m;
-                    const float2 sl2 = make_float2(a.sl2, a.sl2), zz = make_float2(z, z);
+                    const float2 zz = make_float2(z, z);
                     float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {

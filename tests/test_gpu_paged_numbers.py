@@ -1,11 +1,11 @@
 """GPU: attention over a paged cache where numbers leave the ordinary range: infinities in keys and
-values that every row sees."""
+values that every row sees, and very large scores."""
 import math
 
 import pytest
 import torch
 
-from paged_oracle import Case
+from paged_oracle import HALF_STEP, Case
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -92,3 +92,31 @@ def test_scores_and_values_without_an_answer_are_nan(ctx, dtype, new, group):
         got = c.attend(ctx)
         assert torch.isnan(got[:, :group]).all() and torch.isfinite(got[:, group:, :7]).all()
     ctx.sync_check()
+
+
+@pytest.mark.parametrize("dtype,scale", [(F32, 1.0), (F32, 2.0 ** 12), (F16, 0.3), (F16, 11.0), (F16, 2.0 ** 12), (BF16, 0.3), (BF16, 11.0), (BF16, 2.0 ** 12)])
+@pytest.mark.parametrize("new,lens,prefix", [([1], [400], 0), ([40, 150], [300, 2600], 0), ([3, 1], [90, 5], 700), ([60, 70], [60, 300], 700)])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_many_millions_choose_a_key(ctx, dtype, scale, new, lens, prefix, sign):
+    """Scores 2^20 * scale and more apart, far more than what 32 bits round at their size: each row is the value of the key that it scores highest."""
+    c = Case(dtype, new, lens, 1, 2, 64, 16, prefix=prefix, device="cuda", garbage=False)
+    c.q[:], c.k[:] = 0, 0
+    c.q[:, 0, 0], c.q[:, 1, 0] = 2.0 ** 15, 2.0 ** 15 * 1.25
+    places = [(c.prefix_table[j // 16].long(), j % 16) for j in range(prefix)]
+    order = torch.randperm(prefix + max(lens), generator=torch.Generator().manual_seed(2)) % 128  # (several keys have the largest score)
+    for j, (page, slot) in enumerate(places):
+        c.k[page, slot, 0, 0] = sign * 32.0 * (1 + order[j])
+    for b in range(len(lens)):
+        for j in range(lens[b]):
+            page, slot = place(c, b, j)
+            c.k[page, slot, 0, 0] = sign * 32.0 * (1 + order[prefix + j])
+    got = c.attend(ctx, scale=scale).double().cpu()
+    ctx.sync_check()
+    for b in range(len(lens)):
+        k, v = c.keys(b, c.k)[:, 0, 0], c.keys(b, c.v)[:, 0]
+        for i in range(new[b]):
+            n = prefix + lens[b] - new[b] + i + 1
+            top = k[:n] == k[:n].max()
+            # probabilities are equal and exact but for a rounding to the type, which the sum does not have; the sum and mean of few keys
+            want, tol = v[:n][top].mean(0), v[:n][top].abs().mean(0) * (2 * HALF_STEP[dtype] + 2.0 ** -17)
+            assert ((got[c.starts[b] + i] - want).abs() <= tol).all(), (b, i)
