@@ -4,6 +4,7 @@
 #include "common.h"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace petb200 {
 
@@ -70,7 +71,7 @@ struct PagedArgs {
     int hkv = 0, group = 1, dim = 0, causal = 0;
     float sl2 = 0.f; // scale * log2(e): the softmax runs on powers of two
     // Pieces: a row's sum over part of its keys, O unnormalised [piece][hkv][rows][DP] with {m, l} beside it, rows = tokens * group.
-    // m is the largest score * sl2; -inf: the row sees none of these keys, -FLT_MAX: it sees some, all of them at -inf.
+    // m is the largest score * sl2 (less the offset of lifted()); -inf: the row sees none of these keys, -FLT_MAX: it sees some, all of them at -inf.
     float *po = nullptr;
     float2 *pml = nullptr;
     int pieces = 0;     // that paged_join_rows() adds
@@ -99,6 +100,16 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// What a row's powers of two are taken against: its maximum `top` (in powers), less `by` in fp16, whose range of 2^15 above 1 would go unused
+// otherwise.  Probabilities have all their digits down to 2^-14 then and a trace down to 2^-25, of what is 2^by now: with the maximum at
+// 1, keys 17 nats below it would be lost from the sum of v while the sum of the powers has them, and 130 000 such keys are a part
+// of the result that shows.  The sums with v and of the powers are scaled alike, in pieces too, since their m is this one.  (A large maximum
+// is left as it is: the difference would be rounded.)
+constexpr float kLargePower = 1048576.f;
+template <typename T> __device__ __forceinline__ float lifted(float top, float by) {
+    return std::is_same<T, __half>::value && fabsf(top) < kLargePower ? top - by : top;
 }
 
 // Attention of a's tokens over their keys (and the shared ones before them); *need: the workspace that it takes, all that is done where

@@ -315,6 +315,7 @@ template <typename T, int DP> struct RowTile {
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, x));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
         }
+        mx0 = lifted<T>(mx0, 15.f), mx1 = lifted<T>(mx1, 15.f);
         if (__any_sync(0xffffffffu, mx0 > m[0] || mx1 > m[1])) {
             const float n0 = fmaxf(m[0], mx0), n1 = fmaxf(m[1], mx1);
             const float f0 = m[0] == n0 ? 1.f : exp2_approx(m[0] - n0), f1 = m[1] == n1 ? 1.f : exp2_approx(m[1] - n1);

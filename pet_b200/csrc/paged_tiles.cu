@@ -40,7 +40,7 @@ constexpr int kTileRows = 128, kTileKeys = 128, kTileThreads = 512;
 constexpr int kSoftmaxRegs = 176, kOtherRegs = 80;
 static_assert(256 * (kSoftmaxRegs + kOtherRegs) <= kTileThreads * 128, "more registers than the block was launched with: setmaxnreg would wait forever");
 constexpr int kLag = 2; // stages whose copies a fetching thread leaves in flight before it reports the one before them
-constexpr float kGrowth = 8.f, kLargeScore = 1048576.f;
+constexpr float kGrowth = 8.f;
 
 template <int DP> struct TileCfg {
     static constexpr int STAGE = kTileKeys * DP * 2;
@@ -472,7 +472,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                 const int lim = live ? a.s.visible(tok, ql, own, a.causal) - n0 : own_last; // of its own keys (rows past the end: zeros of q, nothing is written)
                 const int warp_lim = __reduce_min_sync(0xffffffffu, lim);
                 const uint32_t lanes = (uint32_t)(warp & 3) << 21, s_t = tmem + lanes + t * 128, o_t = tmem + lanes + 256 + t * 128;
-                float m = -INFINITY, l = 0.f; // m: the maximum in use, times scale log2(e)
+                float m = -INFINITY, l = 0.f; // m: the maximum in use, times scale log2(e), as lifted() leaves it
                 bool ok = true;
                 for (int j = 0; j < steps; ++j) {
                     ok = ptx::mbar_wait_warp(&ctl.s_full[t], j & 1, abort_flag);
@@ -508,7 +508,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                     // Below, a score's product with the scale is not rounded, as m is: of a score t the difference is up to 2^-24 t, which would
                     // be a power out of range where t is large.  Such scores are rounded first.
                     float2 sl2 = make_float2(a.sl2, a.sl2);
-                    if (__any_sync(0xffffffffu, fabsf(top) >= kLargeScore && top > -INFINITY)) {
+                    if (__any_sync(0xffffffffu, fabsf(top) >= kLargePower && top > -INFINITY)) {
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -516,6 +516,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
                                 s[c][i] = __float_as_uint(__uint_as_float(s[c][i]) * a.sl2);
                         sl2 = make_float2(1.f, 1.f);
                     }
+                    top = lifted<T>(top, 7.f); // (and up to 2^8 more while the maximum grows: 2^15 of fp16's 2^16)
                     if (j == 0)
                         m = top;
                     else if (__any_sync(0xffffffffu, top - m > kGrowth || top != top)) {

@@ -1,5 +1,6 @@
 """GPU: attention over a paged cache where numbers leave the ordinary range: infinities in keys and
-values that every row sees, and very large scores."""
+values that every row sees, very large scores, and
+probabilities that 16-bit types hold badly."""
 import math
 
 import pytest
@@ -120,3 +121,72 @@ def test_scores_of_many_millions_choose_a_key(ctx, dtype, scale, new, lens, pref
             # probabilities are equal and exact but for a rounding to the type, which the sum does not have; the sum and mean of few keys
             want, tol = v[:n][top].mean(0), v[:n][top].abs().mean(0) * (2 * HALF_STEP[dtype] + 2.0 ** -17)
             assert ((got[c.starts[b] + i] - want).abs() <= tol).all(), (b, i)
+
+
+# ---- probabilities far below the largest one -------------------------------------------------------------------------------------
+def level_case(dtype, new, lens, top, gap, heads=1, group=1, page=64, prefix=0, **more):
+    """All keys score 0 but key top(b) of each sequence (of the prefix where there is one), which scores `gap` and has v = 0; v = 1 elsewhere."""
+    c = Case(dtype, new, lens, heads, group, 8, page, prefix=prefix, device="cuda", **more)
+    c.q[:], c.k[:], c.v[:] = 0, 0, 1
+    c.q[:, :, 0] = 1
+    for b in range(len(lens)):
+        if prefix:
+            j = top(prefix)
+            p = c.prefix_table[j // page].long(), j % page
+        else:
+            j = top(lens[b])
+            p = place(c, b, j)
+        c.k[p][:, 0], c.v[p] = gap, 0
+    return c
+
+
+def check_level(c, got, gap):
+    """n keys of probability e^-gap beside one of 1.  A probability has a half step of the type relative to itself, or, in fp16, 2^-32 of the
+    row's largest one where that is more (subnormal steps are 2^-24 of values scaled to 2^7 at least); the sum has n / 4 + 64 additions
+    of 32 bits; the power's argument is rounded at gap * log2(e) and the product before it; the result to its type."""
+    u, e = HALF_STEP[c.dtype], math.exp(-gap)
+    for b, n in enumerate(c.lens):
+        n += c.prefix - 1
+        want = n * e / (1 + n * e)
+        tol = want * (u + u + (n / 4 + 64) * 2.0 ** -24 + 4 * gap * 2.0 ** -23 + 2.0 ** -20) + n * 2.0 ** -32 + 2.0 ** -25
+        off = (got[c.starts[b]:c.starts[b + 1]].double().cpu() - want).abs().max()
+        assert off <= tol, f"{float(off):.3g} off {want:.3g}, {tol:.3g} allowed"
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("gap", [9.0, 12.0, 15.0, 16.5, 17.5])
+@pytest.mark.parametrize("top", [lambda n: 0, lambda n: n - 1, lambda n: n // 2], ids=["first", "last", "middle"])
+# clusters, whole units, ranges, draft tokens on very many keys; tiles, tiles split over the keys
+@pytest.mark.parametrize("new,lens,group", [([1], [3000], 1), ([1] * 3000, [250] * 3000, 1), ([1], [130000], 4), ([4, 4], [60000, 130000], 2),
+                                            ([200], [9000], 1), ([30], [130000], 1)])
+def test_keys_far_below_the_largest_keep_their_weight(ctx, dtype, gap, top, new, lens, group):
+    c = level_case(dtype, new, lens, top, gap, group=group, starts=False, garbage=False)
+    got = c.attend(ctx, causal=False, scale=1.0)
+    ctx.sync_check()
+    check_level(c, got, gap)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("gap", [12.0, 16.5, 17.5])
+# a few rows (prefix and own keys in one launch), rows enough for tiles of the prefix, sequences that read it alone
+@pytest.mark.parametrize("seqs,new,own,group", [(3, 1, 500, 1), (40, 1, 300, 4), (4, 60, 2000, 4)])
+def test_keys_far_below_the_largest_behind_a_prefix(ctx, dtype, gap, seqs, new, own, group):
+    c = level_case(dtype, [new] * seqs, [own] * seqs, lambda n: n // 3, gap, group=group, prefix=9000, starts=False, garbage=False)
+    got = c.attend(ctx, causal=False, scale=1.0)
+    ctx.sync_check()
+    check_level(c, got, gap)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new", [1, 130])
+@pytest.mark.parametrize("grows", [5.5, 5.625, 30.0])  # 2^8 is e^5.545: just within what the tiles let a maximum grow, just beyond, far beyond
+def test_a_maximum_that_grows_stays_within_the_type(ctx, dtype, new, grows):
+    """Half of the keys score `grows` above the other half, which come first: probabilities of the type's range until the maximum moves."""
+    c = Case(dtype, [new], [2000], 1, 1, 8, 16, device="cuda", garbage=False)
+    c.q[:], c.k[:], c.v[:] = 0, 0, 1
+    c.q[:, :, 0] = 1
+    for j in range(1000, 2000):
+        p = place(c, 0, j)
+        c.k[p][:, 0], c.v[p] = grows, 2
+    c.check(c.attend(ctx, causal=False, scale=1.0), causal=False, scale=1.0)
+    ctx.sync_check()
