@@ -235,15 +235,16 @@ typedef struct {
  * j + rotary / 2, or 2 j and 2 j + 1 where `interleaved`) is turned by the angle (pos0 + p) * inv_freq[j], formed in 64 bits.
  * inv_freq NULL or rotary 0: nothing is turned.  Sources are of type src_dtype (the cache's, or PETB200_F32), rounded once to the cache's;
  * q_out is of the cache's type.  q NULL: keys and values alone.  Rows outside all sequences, and tokens with p < 0, write nothing to
- * the cache; rows outside all sequences leave q_out as it was.  A page that two sequences of the call both append to is left undefined; q_out must not overlap a source. */
+ * the cache; rows outside all sequences leave q_out as it was.  A page that two sequences of the call both append to is left undefined.
+ * q_out must not overlap a source (PETB200_ERR_INVALID; rows side by side in one merged tensor do not), and no row may lie in the pools. */
 int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const petb200_kv_rows *k,
                           const petb200_kv_rows *v, const petb200_kv_rows *q, const petb200_kv_rows *q_out, int q_heads, int src_dtype,
                           const float *inv_freq, int rotary, int interleaved, int pos0, petb200_stream stream);
 /* out[token, head] = sum_j softmax_j(scale q . k_j) v_j over the token's sequence, query head `head` on key head
  * head / (q_heads / heads).  causal: token i of n sees keys j <= kv_lens[b] - n + i, else all kv_lens[b].  A row that sees no key
  * gives zeros; rows outside all sequences are left as they were; masked and absent keys never contribute, whatever they hold.
- * q and out are of the cache's type, rows 16-byte aligned, and must not overlap; scores, softmax and sums are fp32 (F32 caches: products error-compensated TF32;
- * 16-bit caches: probabilities rounded to the cache's type).  `workspace` is device memory of the size that
+ * q and out are of the cache's type, rows 16-byte aligned, and must not overlap (PETB200_ERR_INVALID), nor out the pools.  Scores, softmax and
+ * sums are fp32 (F32 caches: products error-compensated TF32; 16-bit caches: probabilities rounded to the cache's type).  `workspace` is device memory of the size that
  * petb200_attention_paged_workspace gives for the same call (prefix_len 0), used until the launches have run. */
 int petb200_attention_paged_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const petb200_kv_rows *q,
                                 const petb200_kv_rows *out, int q_heads, int causal, float scale, void *workspace, size_t workspace_bytes,

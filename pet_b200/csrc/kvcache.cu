@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <cstdlib>
 
 namespace petb200 {
 namespace {
@@ -229,6 +230,52 @@ petb200_kv_cache plain_strides(petb200_kv_cache c) {
     return c;
 }
 
+// Whether two sets of rows [tokens, heads, dim] have a byte in common; `bytes` of a row, strides in bytes.  Rows of one merged tensor, side by
+// side in every token, have not, although their ranges meet.  (Ranges that meet with different token strides count as overlapping.)
+struct ByteRows {
+    uintptr_t p;
+    long long tok, head, bytes;
+    int heads;
+};
+bool rows_overlap(ByteRows a, ByteRows b, int tokens) {
+    long long lo[2], hi[2], head_lo[2], head_hi[2]; // of all rows, and of one token's, from a.p
+    ByteRows *r[2] = {&a, &b};
+    const long long apart = (long long)(b.p - a.p);
+    for (int i = 0; i < 2; ++i) {
+        if (tokens <= 1)
+            r[i]->tok = 0;
+        if (r[i]->heads <= 1)
+            r[i]->head = 0;
+        const long long t = r[i]->tok * (tokens - 1), h = r[i]->head * (r[i]->heads - 1), at = i ? apart : 0;
+        head_lo[i] = at + std::min(h, 0ll), head_hi[i] = at + std::max(h, 0ll) + r[i]->bytes;
+        lo[i] = head_lo[i] + std::min(t, 0ll), hi[i] = head_hi[i] + std::max(t, 0ll);
+    }
+    if (lo[0] >= hi[1] || lo[1] >= hi[0])
+        return false;
+    if (a.tok != b.tok)
+        return true;
+    // Whether some token of b, k strides on, reaches into [x, x + n) from [y, y + m).
+    const long long step = std::abs(a.tok);
+    auto meet = [&](long long x, long long n, long long y, long long m) {
+        if (step == 0)
+            return y < x + n && x < y + m;
+        const long long d = x - m - y; // the first k with y + k step > x - m
+        const long long k = d >= 0 ? d / step + 1 : -((-d - 1) / step);
+        return std::max(k, 1ll - tokens) <= tokens - 1 && y + std::max(k, 1ll - tokens) * step < x + n;
+    };
+    if (!meet(head_lo[0], head_hi[0] - head_lo[0], head_lo[1], head_hi[1] - head_lo[1]))
+        return false;
+    for (int i = 0; i < a.heads; ++i)
+        for (int j = 0; j < b.heads; ++j)
+            if (meet(i * a.head, a.bytes, apart + j * b.head, b.bytes))
+                return true;
+    return false;
+}
+bool rows_overlap(const petb200_kv_rows &a, int a_heads, int a_dtype, const petb200_kv_rows &b, int b_heads, int b_dtype, int dim, int tokens) {
+    const long long sa = type_size(a_dtype), sb = type_size(b_dtype);
+    return rows_overlap({(uintptr_t)a.p, a.tok * sa, a.head * sa, dim * sa, a_heads}, {(uintptr_t)b.p, b.tok * sb, b.head * sb, dim * sb, b_heads}, tokens);
+}
+
 int check_cache(petb200_ctx *ctx, const char *what, const petb200_kv_cache *cache, const petb200_kv_seqs *s) {
     if (!cache || !s)
         return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
@@ -351,6 +398,8 @@ int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *ca
     const long long e = 16 / type_size(cache->dtype);
     if (!on_grid(q->p) || !on_grid(out->p) || q->tok % e || q->head % e || out->tok % e || out->head % e || q->tok < 0 || q->head < 0 || out->tok < 0 || out->head < 0)
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
+    if (rows_overlap(*q, q_heads, cache->dtype, *out, q_heads, cache->dtype, cache->dim, seqs->tokens))
+        return fail(ctx, PETB200_ERR_INVALID, "%s: out must not overlap q", what);
     if (!on_grid(workspace))
         return fail(ctx, PETB200_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
     DeviceGuard guard(ctx->device);
@@ -394,6 +443,9 @@ extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *c
     const long long e = 16 / type_size(cache->dtype), es = 16 / type_size(src_dtype);
     if (with_q && (!on_grid(to.p) || to.tok % e || to.head % e || to.tok < 0 || to.head < 0))
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q_out must start on 16-byte boundaries", what);
+    for (int i = 0; with_q && i < 3; ++i)
+        if (rows_overlap(src[i], i ? cache->heads : q_heads, src_dtype, to, q_heads, cache->dtype, cache->dim, seqs->tokens))
+            return fail(ctx, PETB200_ERR_INVALID, "%s: q_out must not overlap a source", what);
     AppendArgs a{};
     a.s = device_seqs(ctx, cache, seqs);
     a.vec = 1;
@@ -449,4 +501,11 @@ extern "C" int petb200_attention_paged_workspace(petb200_ctx *ctx, const petb200
     if (seqs->seqs == 0 || seqs->tokens == 0)
         return PETB200_OK;
     return attend(ctx, cache->dtype, attention_args(ctx, cache, seqs, q_heads), nullptr, prefix_len, nullptr, 0, bytes, nullptr);
+}
+
+// Test hook (not part of the public header): the check of outputs against inputs, on numbers alone.  rows: {address, token stride, head stride,
+// heads, bytes of a row} of either, in bytes.
+extern "C" int petb200_debug_rows_overlap(const long long *a, const long long *b, int tokens) {
+    auto rows = [](const long long *r) { return ByteRows{(uintptr_t)r[0], r[1], r[2], r[4], (int)r[3]}; };
+    return rows_overlap(rows(a), rows(b), tokens);
 }

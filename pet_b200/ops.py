@@ -563,8 +563,8 @@ class Context:
 
         k, v [tokens, heads, dim] (q [tokens, q_heads, dim]): of the cache's type, or fp32, rounded once; views of a merged projection are
         read in place.  k_cache, v_cache [pages, page_size, heads, dim], fp32, fp16 or bf16, any page, slot and head strides that are
-        multiples of 16 bytes; dim a multiple of 8 up to 128; q_out must not overlap a source.  page_table [seqs, width] int32: the pages of each sequence in order.  kv_lens
-        [seqs] int32: its keys, the new ones among them, which are the last.  q_starts [seqs + 1] int32: its tokens are rows
+        multiples of 16 bytes; dim a multiple of 8 up to 128; q_out must not overlap a source.  page_table [seqs, width] int32: the pages of
+        each sequence in order.  kv_lens [seqs] int32: its keys, the new ones among them, which are the last.  q_starts [seqs + 1] int32: its tokens are rows
         q_starts[b] .. q_starts[b + 1] - 1 (rows behind the last sequence write nothing); None: as many for each.
         inv_freq [pairs] fp32: pair j is turned by (pos0 + position) * inv_freq[j], the first 2 * pairs values of a head: j with
         j + pairs, or 2 j with 2 j + 1 (interleaved); None: nothing is turned.  No two sequences may append to one page."""
@@ -593,8 +593,6 @@ class Context:
                 so = self._kv_rows("q_out", q_out, tokens, q_heads, dim, dtype)
                 if so[2] != 1:
                     raise L.PetError(L.ERR_UNSUPPORTED, "q_out: the values of a head must be contiguous")
-                if q_out.data_ptr() == q.data_ptr():
-                    raise L.PetError(L.ERR_INVALID, "q_out must not overlap q")
             q_rows, out_rows = L.KV_ROWS.pack(q.data_ptr(), sq[0], sq[1]), L.KV_ROWS.pack(q_out.data_ptr(), so[0], so[1])
         elif q_out is not None:
             raise L.PetError(L.ERR_INVALID, "q_out without q")
@@ -653,7 +651,8 @@ class Context:
         Cache, page_table, kv_lens and q_starts as for kv_append (which puts the tokens' own keys there first); q_heads is a multiple of the
         cache's heads, query head h reads key head h // (q_heads // heads).  causal: a token sees the keys up to its own; else all
         kv_lens[b].  scale: None is dim ** -0.5.  A token that sees no key gives zeros; rows behind the last sequence are left as they
-        were (with out=None: unset).  Any page size, one token or many; lengths are read on the device, so the call can be captured."""
+        were (with out=None: unset); out must not overlap q.  Any page size, one token or many; lengths are read on the device, so the call
+        can be captured."""
         return self._kv_attention(q, k_cache, v_cache, None, 0, page_table, kv_lens, q_starts, causal, scale, out)
 
     def attention_prefix(self, q, k_cache, v_cache, prefix_table, prefix_len, page_table, kv_lens, q_starts=None, causal=True, scale=None, out=None):

@@ -1,0 +1,54 @@
+"""GPU: calls of the paged cache as the documentation allows them, at its edges: outputs beside and over inputs, empty calls."""
+import pytest
+import torch
+
+from paged_oracle import Case
+from pet_b200.lib import ERR_INVALID, PetError
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def arguments(c):
+    return c.pool(c.k), c.pool(c.v), c.on(c.table), torch.tensor(c.lens, dtype=torch.int32, device="cuda")
+
+
+def test_empty_calls_with_outputs(ctx):
+    c = Case(BF16, [1, 1], [20, 30], 2, 2, 64, device="cuda", starts=False)
+    k, v, t, n = arguments(c)
+    q, buf = c.on(c.q), torch.full((4, 4, 64), 3.0, device="cuda", dtype=BF16)
+    none, before = q[:0], (k.clone(), v.clone())
+    assert ctx.kv_append(none[:, :2], none[:, 2:], k, v, t[:0], n[:0], q=none, q_out=buf[:0]).shape == (0, 4, 64)
+    assert ctx.attention_paged(none, k, v, t[:0], n[:0], out=buf[:0]).shape == (0, 4, 64)
+    starts = torch.zeros(3, dtype=torch.int32, device="cuda")  # sequences without tokens
+    assert ctx.kv_append(none[:, :2], none[:, 2:], k, v, t, n, q_starts=starts, q=none, q_out=buf[:0]).shape == (0, 4, 64)
+    assert ctx.attention_paged(none, k, v, t, n, q_starts=starts, out=buf[:0]).shape == (0, 4, 64)
+    ctx.sync_check()
+    assert (buf == 3).all() and all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip((k, v), before))
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_outputs_beside_and_over_inputs(ctx, new):
+    c = Case(BF16, [new, new], [60, 80], 2, 2, 64, device="cuda", starts=False)
+    k, v, t, n = arguments(c)
+
+    def refused(call):
+        with pytest.raises(PetError, match="overlap") as e:
+            call()
+        assert e.value.status == ERR_INVALID
+    both = torch.zeros(c.tokens + 1, 12, 64, device="cuda", dtype=BF16)
+    q = both[:-1, :4]
+    q.copy_(c.on(c.q))
+    for out in (both[:-1, :4], both[:-1, 3:7], both[1:, :4], both[1:, 1:5], both.view(-1, 4, 64)[:c.tokens]):
+        refused(lambda: ctx.attention_paged(q, k, v, t, n, out=out))
+    c.check(ctx.attention_paged(q, k, v, t, n, out=both[:-1, 4:8]))  # side by side in each token
+    c.check(ctx.attention_paged(q, k, v, t, n, out=both[1:, 8:12]))
+    ctx.sync_check()
+    # appending: queries, keys and values of a merged projection, the turned queries beside them
+    for out in (both[:-1, :4], both[:-1, 3:7], both[:-1, 6:10], both[1:, 5:9]):
+        refused(lambda: ctx.kv_append(both[:-1, 4:6], both[:-1, 6:8], k, v, t, n, q=q, q_out=out))
+    got = ctx.kv_append(both[:-1, 4:6], both[:-1, 6:8], k, v, t, n, q=q, q_out=both[:-1, 8:])
+    ctx.sync_check()
+    assert torch.equal(got, q) and got.data_ptr() == both[:, 8:].data_ptr()
+    wide = torch.zeros(c.tokens, 8, 64, device="cuda")  # fp32 sources, the queries' halves inside their memory
+    refused(lambda: ctx.kv_append(wide[:, 4:6], wide[:, 6:], k, v, t, n, q=wide[:, :4], q_out=wide.view(BF16).view(c.tokens, 16, 64)[:, 12:]))
