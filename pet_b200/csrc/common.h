@@ -59,6 +59,7 @@ struct petb200_ctx {
     };
     std::vector<BandTcPlan> band_tc;
     void (*band_tc_destroy)(void *) = nullptr;
+    int paged_starve = 0; // test hook, see petb200_debug_paged_starve
     std::vector<const void *> smem_raised; // kernels whose shared-memory limit raise_smem() has set on this device
     ~petb200_ctx() {
         for (void *p : band_retired)

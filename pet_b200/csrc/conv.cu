@@ -447,9 +447,9 @@ int MatmulPlan::bench_launch(cudaStream_t s) {
 } // namespace petb200
 
 // Test hooks for the give-up path of the tensor-core kernel's bounded waits (not part of the public header).
-// set_wait_limit: how long a wait on an mbarrier may last on the current device (default 2 s).  conv_starve: while on,
-// the plan's filter producer announces 64 bytes more per stage than it loads — a flag that nothing sets — so the MMA
-// warp's wait runs out, every role leaves through its abort path, and petb200_check_device_status reports
+// set_wait_limit: how long a wait on an mbarrier may last on the current device (default 2 s), in every kernel that has such waits.
+// conv_starve: while on, the plan's filter producer announces 64 bytes more per stage than it loads — a flag that nothing sets — so the
+// MMA warp's wait runs out, every role leaves through its abort path, and petb200_check_device_status reports
 // PETB200_ERR_DEVICE.  Nothing faults and nothing hangs: the kernel returns after the limit.
 extern "C" int petb200_debug_set_wait_limit(unsigned long long ns) { return petb200::tc_set_wait_limit_ns(ns); }
 extern "C" int petb200_debug_conv_starve(petb200_plan *plan, int on) {

@@ -1900,6 +1900,7 @@ int igemm_tf32_wait_limit(unsigned long long ns);
 int igemm_f16_wait_limit(unsigned long long ns);
 int igemm_opt_wait_limit(unsigned long long ns);
 int igemm_band_wait_limit(unsigned long long ns);
+int paged_tiles_wait_limit(unsigned long long ns); // (paged_tiles.cu)
 #define PETB200_IGEMM_PICK(NAME, MATH)                                                                                            \
     KernelFn NAME(bool a_kmajor, int pp) {                                                                                          \
         if (a_kmajor)                                                                                                               \

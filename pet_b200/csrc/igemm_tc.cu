@@ -1166,7 +1166,7 @@ void tc_conv_out_dims(void *h, int *d5) {
 }
 void tc_conv_set_starve(void *h, int on) { ((TcConv *)h)->full.starve = on; }
 int tc_set_wait_limit_ns(unsigned long long ns) {
-    for (SetWaitLimitFn set : {igemm_tf32_wait_limit, igemm_f16_wait_limit, igemm_opt_wait_limit, igemm_band_wait_limit})
+    for (SetWaitLimitFn set : {igemm_tf32_wait_limit, igemm_f16_wait_limit, igemm_opt_wait_limit, igemm_band_wait_limit, paged_tiles_wait_limit})
         if (int rc = set(ns))
             return rc;
     return PETB200_OK;

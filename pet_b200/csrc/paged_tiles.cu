@@ -110,7 +110,7 @@ template <typename T> __device__ __forceinline__ uint32_t word_clean(uint32_t w)
 }
 
 template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
-    k_paged_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedArgs a, int splits, int to_pieces, int tma) {
+    k_paged_tiles(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PagedArgs a, int splits, int to_pieces, int tma, int starve) {
     using C = TileCfg<DP>;
     extern __shared__ __align__(1024) unsigned char smem[];
     int2 *row_table = reinterpret_cast<int2 *>(smem + C::Q + C::NS * C::STAGE); // [2][128]: a tile's keys as {page (-1: zeros), slot}
@@ -128,7 +128,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
         ptx::mbar_init(&ctl.q_full, tma ? 96 : 128);
         ptx::mbar_init(&ctl.raw, 1);
         for (int i = 0; i < C::NS; ++i) {
-            ptx::mbar_init(&ctl.full[i], tma ? 1 : 128);
+            ptx::mbar_init(&ctl.full[i], (tma ? 1 : 128) + starve); // (starve, a test hook: an arrival that never comes)
             ptx::mbar_init(&ctl.empty[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
@@ -679,7 +679,7 @@ int tiles_launch(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_b
         return rc;
     CUtensorMap kmap{}, vmap{};
     const int tma = page_map<T>(a, a.kc, a.kp, a.ks, a.kh, kmap) && page_map<T>(a, a.vc, a.vp, a.vs, a.vh, vmap);
-    launch_pdl(k_paged_tiles<T, DP>, dim3((unsigned)(units * splits)), kTileThreads, C::SMEM, s, kmap, vmap, a, splits, (int)(pieces_out || splits > 1), tma);
+    launch_pdl(k_paged_tiles<T, DP>, dim3((unsigned)(units * splits)), kTileThreads, C::SMEM, s, kmap, vmap, a, splits, (int)(pieces_out || splits > 1), tma, ctx->paged_starve);
     int rc = launched(ctx, "k_paged_tiles");
     if (rc || pieces_out || splits == 1)
         return rc;
@@ -687,6 +687,10 @@ int tiles_launch(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t ws_b
 }
 
 } // namespace
+
+int paged_tiles_wait_limit(unsigned long long ns) {
+    return cudaMemcpyToSymbol(ptx::g_mbar_wait_limit_ns, &ns, sizeof ns) == cudaSuccess ? PETB200_OK : PETB200_ERR_CUDA;
+}
 
 int paged_tiles_pieces(petb200_ctx *ctx, const PagedArgs &a) {
     const bool one = a.s.kv_lens == nullptr;
@@ -706,3 +710,12 @@ int paged_tiles_run(petb200_ctx *ctx, int dtype, PagedArgs a, char *ws, size_t w
 }
 
 } // namespace petb200
+
+// Test hook for the give-up path of k_paged_tiles (not part of the public header; petb200_debug_set_wait_limit shortens the wait): while on, the
+// stages of its ring expect one arrival more than there are, so the products' wait runs out, every role leaves and the status word says so.
+extern "C" int petb200_debug_paged_starve(petb200_ctx *ctx, int on) {
+    if (!ctx)
+        return PETB200_ERR_INVALID;
+    ctx->paged_starve = on != 0;
+    return PETB200_OK;
+}

@@ -52,3 +52,33 @@ def test_outputs_beside_and_over_inputs(ctx, new):
     assert torch.equal(got, q) and got.data_ptr() == both[:, 8:].data_ptr()
     wide = torch.zeros(c.tokens, 8, 64, device="cuda")  # fp32 sources, the queries' halves inside their memory
     refused(lambda: ctx.kv_append(wide[:, 4:6], wide[:, 6:], k, v, t, n, q=wide[:, :4], q_out=wide.view(BF16).view(c.tokens, 16, 64)[:, 12:]))
+
+
+# Keys by TMA and by copies, tiles that split their keys, the shared prefix in tiles; fewer keys than the ring's stages hold, and many more
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("new,lens,prefix", [([150, 40], [150, 300], 0), ([100], [5000], 0), ([1] * 40, [90] * 40, 2000)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_wait_that_runs_out_is_reported(ctx, page, new, lens, prefix, dim):
+    """A ring whose stages expect an arrival that never comes, waits of 5 ms: the call returns, says so once, and the next one is right."""
+    import ctypes as C
+    import time
+    from pet_b200 import lib as L
+    lib = L.load()
+    lib.petb200_debug_set_wait_limit.argtypes = [C.c_ulonglong]
+    lib.petb200_debug_paged_starve.argtypes = [C.c_void_p, C.c_int]
+    c = Case(BF16, new, lens, 1, 4, dim, page, prefix=prefix, device="cuda")
+    c.check(c.attend(ctx))
+    ctx.sync_check()
+    assert lib.petb200_debug_set_wait_limit(5_000_000) == 0
+    try:
+        assert lib.petb200_debug_paged_starve(ctx.h, 1) == 0
+        began = time.monotonic()
+        c.attend(ctx)
+        with pytest.raises(PetError, match="wait") as e:
+            ctx.sync_check()
+        assert e.value.status == L.ERR_DEVICE and time.monotonic() - began < 1.5  # (the unshortened wait is 2 s)
+    finally:
+        lib.petb200_debug_paged_starve(ctx.h, 0)
+        assert lib.petb200_debug_set_wait_limit(2_000_000_000) == 0
+    c.check(c.attend(ctx))
+    ctx.sync_check()
