@@ -92,10 +92,9 @@ extern "C" int petb200_check_device_status(petb200_ctx *ctx, petb200_stream stre
     PETB200_CUDA(ctx, cudaMemcpy(&v, ctx->d_status, sizeof v, cudaMemcpyDeviceToHost));
     if (v) {
         cudaMemset(ctx->d_status, 0, sizeof v);
-        if (v & 2) // kStatusPage
-            return fail(ctx, PETB200_ERR_DEVICE,
-                        "a page table names a page outside the cache, or a sequence has more keys than its row of the table has pages for (status %d)", v);
-        return fail(ctx, PETB200_ERR_DEVICE, "a kernel gave up on a bounded wait (status %d)", v);
+        const char *page = v & kStatusPage ? "a page table names a page outside the cache, or a sequence has more keys than its row of the table has pages for" : "";
+        const char *wait = v & kStatusWait ? "a kernel gave up on a bounded wait" : "";
+        return fail(ctx, PETB200_ERR_DEVICE, "%s%s%s (status %d)", wait, *page && *wait ? "; " : "", page, v);
     }
     return PETB200_OK;
 }

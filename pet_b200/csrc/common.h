@@ -35,6 +35,9 @@ struct DevBuf {
         return e;
     }
 };
+// Bits of the context's status word: a wait that ran out, and what the lengths and tables of a paged cache may get wrong (a page outside the
+// cache, or a sequence with more keys than its row of the table has pages for).
+constexpr int kStatusWait = 1, kStatusPage = 2;
 } // namespace petb200
 
 struct petb200_ctx {
@@ -44,7 +47,7 @@ struct petb200_ctx {
     size_t smem_optin = 0;
     uint64_t launches = 0;
     std::string err;
-    int *d_status = nullptr; // device word kernels write when a bounded wait expires
+    int *d_status = nullptr; // device word of kStatus* bits that kernels set
     bool band_attr_set = false;   // the banded-product kernel's shared-memory limit was raised on this device
     bool tc_attr_set = false;     // the same for the tensor-core kernel and its preparation
     int cluster_slots[17] = {0};  // clusters of that many of its CTAs that the device holds (0: not asked yet)

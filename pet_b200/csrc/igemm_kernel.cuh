@@ -1877,7 +1877,7 @@ k_igemm(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUte
         while (ptx::globaltimer_ns() - t0 < 200000ull)
             __nanosleep(1000);
         if (threadIdx.x == 0 && P.status)
-            atomicExch(P.status, 1);
+            atomicOr(P.status, kStatusWait);
     }
     ptx::tc_fence_before();
     __syncthreads();

@@ -9,8 +9,6 @@
 namespace petb200 {
 
 constexpr int kPagedMaxDim = 128; // head widths served: multiples of 8 up to this (a row is whole 16-byte pieces)
-// Bits of the context's status word besides 1 (a wait that ran out): what the lengths and tables on the device may get wrong.
-constexpr int kStatusPage = 2; // a page outside the cache, or a sequence with more keys than its row of the table has pages for
 
 // Sequences of one call.  Lengths and tables live on the device; the host knows only how much there can be.
 struct PagedSeqs {

@@ -120,7 +120,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
     volatile int *abort_flag = &ctl.abort;
     if (q_s & 1023) { // (the swizzle counts from 1024-byte boundaries; a block's dynamic memory begins on one)
         if (threadIdx.x == 0)
-            atomicOr(a.s.status, 1);
+            atomicOr(a.s.status, kStatusWait);
         return;
     }
 
@@ -624,7 +624,7 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
         while (ptx::globaltimer_ns() - t < 200000ull)
             __nanosleep(1000);
         if (threadIdx.x == 0)
-            atomicOr(a.s.status, 1);
+            atomicOr(a.s.status, kStatusWait);
     }
     ptx::tc_fence_before();
     __syncthreads();

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from paged_oracle import Case
-from pet_b200.lib import ERR_INVALID, PetError
+from pet_b200.lib import ERR_DEVICE, ERR_INVALID, PetError
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -54,18 +54,24 @@ def test_outputs_beside_and_over_inputs(ctx, new):
     refused(lambda: ctx.kv_append(wide[:, 4:6], wide[:, 6:], k, v, t, n, q=wide[:, :4], q_out=wide.view(BF16).view(c.tokens, 16, 64)[:, 12:]))
 
 
+def hooks():
+    import ctypes as C
+    from pet_b200 import lib as L
+    lib = L.load()
+    lib.petb200_debug_set_wait_limit.argtypes = [C.c_ulonglong]
+    lib.petb200_debug_paged_starve.argtypes = [C.c_void_p, C.c_int]
+    lib.petb200_debug_conv_starve.argtypes = [C.c_void_p, C.c_int]
+    return lib
+
+
 # Keys by TMA and by copies, tiles that split their keys, the shared prefix in tiles; fewer keys than the ring's stages hold, and many more
 @pytest.mark.parametrize("page", [16, 7])
 @pytest.mark.parametrize("new,lens,prefix", [([150, 40], [150, 300], 0), ([100], [5000], 0), ([1] * 40, [90] * 40, 2000)])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_a_wait_that_runs_out_is_reported(ctx, page, new, lens, prefix, dim):
     """A ring whose stages expect an arrival that never comes, waits of 5 ms: the call returns, says so once, and the next one is right."""
-    import ctypes as C
     import time
-    from pet_b200 import lib as L
-    lib = L.load()
-    lib.petb200_debug_set_wait_limit.argtypes = [C.c_ulonglong]
-    lib.petb200_debug_paged_starve.argtypes = [C.c_void_p, C.c_int]
+    lib = hooks()
     c = Case(BF16, new, lens, 1, 4, dim, page, prefix=prefix, device="cuda")
     c.check(c.attend(ctx))
     ctx.sync_check()
@@ -76,9 +82,37 @@ def test_a_wait_that_runs_out_is_reported(ctx, page, new, lens, prefix, dim):
         c.attend(ctx)
         with pytest.raises(PetError, match="wait") as e:
             ctx.sync_check()
-        assert e.value.status == L.ERR_DEVICE and time.monotonic() - began < 1.5  # (the unshortened wait is 2 s)
+        assert e.value.status == ERR_DEVICE and time.monotonic() - began < 1.5  # (the unshortened wait is 2 s)
     finally:
         lib.petb200_debug_paged_starve(ctx.h, 0)
         assert lib.petb200_debug_set_wait_limit(2_000_000_000) == 0
     c.check(c.attend(ctx))
+    ctx.sync_check()
+
+
+@pytest.mark.parametrize("last", ["attention", "convolution"])
+def test_a_bad_page_and_a_wait_that_runs_out_are_both_reported(ctx, last):
+    lib = hooks()
+    c = Case(BF16, [1, 1], [60, 80], 2, 2, 64, device="cuda", garbage=False)
+    c.table[1, 2] = -5
+    tiles = Case(BF16, [150], [150], 1, 2, 64, device="cuda")
+    x, w = torch.randn(1, 64, 28, 28, device="cuda"), torch.randn(64, 64, 3, 3, device="cuda")
+    plan = ctx.conv2d_plan(x.shape, w.shape, 1, 1)
+    ctx.conv2d_set_weights(plan, w)
+    assert lib.petb200_debug_set_wait_limit(5_000_000) == 0
+    try:
+        c.attend(ctx)
+        if last == "attention":
+            assert lib.petb200_debug_paged_starve(ctx.h, 1) == 0
+            tiles.attend(ctx)
+        else:
+            assert lib.petb200_debug_conv_starve(plan.h, 1) == 0
+            ctx.conv2d_run(plan, x)
+        with pytest.raises(PetError, match="wait.*page") as e:
+            ctx.sync_check()
+        assert e.value.status == ERR_DEVICE
+    finally:
+        lib.petb200_debug_paged_starve(ctx.h, 0)
+        lib.petb200_debug_conv_starve(plan.h, 0)
+        assert lib.petb200_debug_set_wait_limit(2_000_000_000) == 0
     ctx.sync_check()
