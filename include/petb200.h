@@ -219,7 +219,8 @@ typedef struct {
  * kv_lens[b] counts its keys with those of the tokens of this call, which are its last ones.  q_starts (seqs + 1 entries) gives its
  * tokens as rows [q_starts[b], q_starts[b + 1]); NULL: every sequence has tokens / seqs of them.  The three arrays live on the device and are
  * read when the kernels run.  Table entries past a sequence's keys are not read.  A page outside the cache counts as zeros, keys past the
- * table's width are left out, and petb200_check_device_status reports either. */
+ * table's width are left out, and petb200_check_device_status reports either.  q_starts that run backwards or past the tokens give some
+ * tokens to no sequence or to several, whose rows are then undefined; the attentions report more tokens than the call has. */
 typedef struct {
     const int *page_table, *kv_lens, *q_starts;
     long long table_stride;

@@ -93,8 +93,9 @@ extern "C" int petb200_check_device_status(petb200_ctx *ctx, petb200_stream stre
     if (v) {
         cudaMemset(ctx->d_status, 0, sizeof v);
         const char *page = v & kStatusPage ? "a page table names a page outside the cache, or a sequence has more keys than its row of the table has pages for" : "";
+        const char *starts = v & kStatusStarts ? "q_starts that run backwards: its sequences have more tokens than the call" : "";
         const char *wait = v & kStatusWait ? "a kernel gave up on a bounded wait" : "";
-        return fail(ctx, PETB200_ERR_DEVICE, "%s%s%s (status %d)", wait, *page && *wait ? "; " : "", page, v);
+        return fail(ctx, PETB200_ERR_DEVICE, "%s%s%s%s%s (status %d)", wait, *wait && v != kStatusWait ? "; " : "", page, *page && *starts ? "; " : "", starts, v);
     }
     return PETB200_OK;
 }

@@ -35,9 +35,9 @@ struct DevBuf {
         return e;
     }
 };
-// Bits of the context's status word: a wait that ran out, and what the lengths and tables of a paged cache may get wrong (a page outside the
-// cache, or a sequence with more keys than its row of the table has pages for).
-constexpr int kStatusWait = 1, kStatusPage = 2;
+// Bits of the context's status word: a wait that ran out, and what the lengths, tables and starts of a paged cache may get wrong (a page outside
+// the cache, or a sequence with more keys than its row of the table has pages for; sequences that have more tokens together than the call).
+constexpr int kStatusWait = 1, kStatusPage = 2, kStatusStarts = 4;
 } // namespace petb200
 
 struct petb200_ctx {

@@ -94,6 +94,8 @@ template <typename T> __device__ __forceinline__ bool finite(T v) {
     return fabsf(f) <= FLT_MAX;
 }
 
+// a + b, at most 2^32 - 1: starts that run backwards may claim any amount of work, and a sum that wrapped round would place it wrongly.
+__device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) { return a + min(b, ~a); }
 // Sum of `x` over the threads before this one, and over all of them in `total`.
 __device__ __forceinline__ unsigned block_scan(unsigned x, unsigned &total, unsigned *tmp) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -101,20 +103,21 @@ __device__ __forceinline__ unsigned block_scan(unsigned x, unsigned &total, unsi
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
-        inc += lane >= o ? v : 0u;
+        inc = add_sat(inc, lane >= o ? v : 0u);
     }
     __syncthreads(); // (tmp of an earlier scan has been read)
     if (lane == 31)
         tmp[warp] = inc;
+    const unsigned up = __shfl_up_sync(0xffffffffu, inc, 1);
     __syncthreads();
-    unsigned before = 0;
+    unsigned before = lane ? up : 0u;
     total = 0;
 #pragma unroll
     for (int w = 0; w < kRowWarps; ++w) {
-        before += w < warp ? tmp[w] : 0u;
-        total += tmp[w];
+        before = add_sat(before, w < warp ? tmp[w] : 0u);
+        total = add_sat(total, tmp[w]);
     }
-    return before + inc - x;
+    return before;
 }
 
 enum { kModeRanges = 0, kModeUnits = 1, kModePieces = 2, kModeCluster = 3 };
@@ -535,9 +538,9 @@ __device__ __forceinline__ void fma4(float4 &x, float w, float4 y) {
     x.x = fmaf(w, y.x, x.x), x.y = fmaf(w, y.y, x.y), x.z = fmaf(w, y.z, x.z), x.w = fmaf(w, y.w, x.w);
 }
 
-// FEW > 0 (fp32): no tile has more than that many rows.
+// FEW > 0 (fp32): no tile has more than that many rows.  most: of the sequences' steps (units where they are whole) there can be so many.
 template <typename T, int DP, int FEW>
-__global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int own_mode, int prefix_blocks, int prefix_pieces, int cluster) {
+__global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows(const PagedArgs a, int own_mode, unsigned most, int prefix_blocks, int prefix_pieces, int cluster) {
     using C = RowCfg<T, DP>;
     using Loader = RowTile<T, DP>;
     using Tile = typename std::conditional<FEW == 0, RowTile<T, DP>, FewRows<DP, FEW ? FEW : 1>>::type;
@@ -578,12 +581,23 @@ __global__ void __launch_bounds__(kRowThreads, RowCfg<T, DP>::CTAS) k_paged_rows
     for (int b0 = 0; b0 < seqs; b0 += kRowThreads) {
         unsigned t;
         block_scan(b0 + (int)threadIdx.x < seqs ? cost_of(b0 + threadIdx.x) : 0u, t, tmp);
-        total += t;
+        total = add_sat(total, t);
     }
     const unsigned G = mode == kModeRanges ? min(grid, total) : total;
     if (mode == kModeRanges && threadIdx.x == 0 && a.meta)
         a.meta[cta] = make_int4(-1, 0, 0, 0);
-    if (cta >= G)
+    if (a.s.q_starts && (int)blockIdx.x == prefix_blocks) { // (one block says so, of any excess; beyond `most` nothing is done)
+        unsigned tokens = 0;
+        for (int b0 = 0; b0 < seqs; b0 += kRowThreads) {
+            unsigned t;
+            int t0;
+            block_scan(b0 + (int)threadIdx.x < seqs ? (unsigned)a.s.span(b0 + threadIdx.x, t0) : 0u, t, tmp);
+            tokens = add_sat(tokens, t);
+        }
+        if (tokens > (unsigned)a.s.tokens && threadIdx.x == 0)
+            atomicOr(a.s.status, kStatusStarts);
+    }
+    if (cta >= G || (!one && total > most))
         return;
     // whole units are taken from the last one down: later rows of a prompt see more keys
     const unsigned begin = mode == kModeRanges ? (unsigned)((unsigned long long)cta * total / G) : total - 1 - cta;
@@ -975,10 +989,11 @@ int rows_launch_as(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, siz
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr, cfg.numAttrs = pdl_enabled() ? 2 : 1;
-        (void)cudaLaunchKernelEx(&cfg, k_paged_rows<T, DP, FEW>, a, mode, 0, 1, cluster);
+        (void)cudaLaunchKernelEx(&cfg, k_paged_rows<T, DP, FEW>, a, mode, (unsigned)units, 0, 1, cluster);
         return launched(ctx, "k_paged_rows");
     }
-    launch_pdl(k_paged_rows<T, DP, FEW>, dim3(grid + (unsigned)prefix_blocks), kRowThreads, C::SMEM, s, a, mode, (int)prefix_blocks, std::max(1, n_prefix), 1);
+    launch_pdl(k_paged_rows<T, DP, FEW>, dim3(grid + (unsigned)prefix_blocks), kRowThreads, C::SMEM, s, a, mode,
+               (unsigned)(mode == kModeRanges ? units * steps : units), (int)prefix_blocks, std::max(1, n_prefix), 1);
     int rc = launched(ctx, "k_paged_rows");
     if (rc || mode != kModeRanges)
         return rc;

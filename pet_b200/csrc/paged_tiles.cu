@@ -196,6 +196,15 @@ template <typename T, int DP> __global__ void __launch_bounds__(kTileThreads, 1)
             }
         }
     }
+    if (warp == 12 && blockIdx.x == 0 && !one && a.s.q_starts) { // (one block says that the starts run backwards)
+        unsigned long long tokens = 0;
+        for (int b0 = lane, t0; b0 < a.s.seqs; b0 += 32)
+            tokens += (unsigned)a.s.span(b0, t0);
+        for (int o = 16; o > 0; o >>= 1)
+            tokens += __shfl_xor_sync(0xffffffffu, tokens, o);
+        if (tokens > (unsigned long long)a.s.tokens && lane == 0)
+            atomicOr(a.s.status, kStatusStarts);
+    }
     __syncthreads();
     const uint32_t tmem = ctl.tmem;
     const int b = ctl.b;

@@ -116,3 +116,61 @@ def test_a_bad_page_and_a_wait_that_runs_out_are_both_reported(ctx, last):
         lib.petb200_debug_conv_starve(plan.h, 0)
         assert lib.petb200_debug_set_wait_limit(2_000_000_000) == 0
     ctx.sync_check()
+
+
+def told(ctx):
+    """What the device has to say of the calls so far."""
+    try:
+        ctx.sync_check()
+    except PetError as e:
+        assert e.status == ERR_DEVICE
+        return str(e)
+    return ""
+
+
+LARGE, SMALL = 2 ** 31 - 1, -2 ** 31
+BAD_STARTS = [[-7, 900, 3, 4], [5, 2, 4, 1], [LARGE, SMALL, 3, LARGE], [0, LARGE, 0, LARGE], [SMALL, SMALL, SMALL, SMALL], [3, 3, 3, 2], [1, 0, 9, 0]]
+
+
+# rows on a cluster, in ranges, as whole units; tiles, split and not; a prefix read together and alone
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new,keys,group,prefix", [(2, 60, 2, 0), (3, 9000, 2, 0), (2, 40, 40, 0), (60, 300, 3, 0), (40, 5000, 2, 0), (2, 60, 2, 700), (80, 90, 2, 700)])
+def test_bad_starts_reach_no_other_memory(ctx, dtype, new, keys, group, prefix):
+    """Starts that run backwards or past the tokens: whatever the result, nothing outside the call's rows and the sequences' pages is written."""
+    c = Case(dtype, [new] * 3, [keys] * 3, 2, group, 64, 16, prefix=prefix, device="cuda", garbage=False)
+    k, v, t, n = arguments(c)
+    before, named = (k.clone(), v.clone()), torch.zeros(k.shape[0], dtype=torch.bool, device="cuda")
+    named[t[:, :-(-keys // 16)].flatten().long()] = True
+    heads, rows = 2 * group, slice(3, 3 + c.tokens)
+    big = [torch.full((c.tokens + 6, heads, 64), 7.0, dtype=dtype, device="cuda") for _ in range(3)]
+    q, out, q_out = (b[rows] for b in big)
+    q.copy_(c.on(c.q))
+    for starts in BAD_STARTS:
+        s = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        if prefix:
+            ctx.attention_prefix(q, k, v, c.on(c.prefix_table), prefix, t, n, q_starts=s, out=out)
+        else:
+            ctx.attention_paged(q, k, v, t, n, q_starts=s, out=out)
+        assert "page" not in told(ctx)
+        ctx.kv_append(q[:, :2], q[:, 2:4], k, v, t, n, q_starts=s, q=q, q_out=q_out, inv_freq=torch.ones(16, device="cuda"), pos0=prefix)
+        assert told(ctx) == ""
+        for b in big:
+            assert (b[:3] == 7).all() and (b[-3:] == 7).all()
+        assert torch.equal(k[~named], before[0][~named]) and torch.equal(v[~named], before[1][~named])
+    s = c.on(c.q_starts)  # the same memory, in order
+    k.copy_(before[0]), v.copy_(before[1])
+    c.check(c.attend(ctx))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new,keys,group", [(8, 60, 8), (8, 9000, 4), (16, 40, 40), (300, 300, 2), (100, 5000, 4)])
+def test_starts_that_claim_more_rows_than_there_are(ctx, dtype, new, keys, group):
+    """Sequences that have the tokens of others too, more together than the call: told once, and the next call is right."""
+    c = Case(dtype, [new] * 8, [keys] * 8, 1, group, 64, 16, device="cuda", garbage=False, width=-(-keys // 16))
+    k, v, t, n = arguments(c)
+    q = c.on(c.q)
+    s = torch.tensor([0, c.tokens] * 4 + [0], dtype=torch.int32, device="cuda")
+    ctx.attention_paged(q, k, v, t, n, q_starts=s)
+    assert "q_starts" in told(ctx)
+    assert told(ctx) == ""
+    c.check(c.attend(ctx))
