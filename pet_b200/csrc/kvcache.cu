@@ -229,6 +229,14 @@ petb200_kv_cache plain_strides(petb200_kv_cache c) {
         c.k_head = c.v_head = 0;
     return c;
 }
+petb200_kv_rows plain_strides(const petb200_kv_rows *rows, int tokens, int heads) {
+    petb200_kv_rows r = rows ? *rows : petb200_kv_rows{};
+    if (tokens <= 1)
+        r.tok = 0;
+    if (heads <= 1)
+        r.head = 0;
+    return r;
+}
 
 // Whether two sets of rows [tokens, heads, dim] have a byte in common; `bytes` of a row, strides in bytes.  Rows of one merged tensor, side by
 // side in every token, have not, although their ranges meet.  (Ranges that meet with different token strides count as overlapping.)
@@ -239,13 +247,9 @@ struct ByteRows {
 };
 bool rows_overlap(ByteRows a, ByteRows b, int tokens) {
     long long lo[2], hi[2], head_lo[2], head_hi[2]; // of all rows, and of one token's, from a.p
-    ByteRows *r[2] = {&a, &b};
+    const ByteRows *r[2] = {&a, &b};
     const long long apart = (long long)(b.p - a.p);
     for (int i = 0; i < 2; ++i) {
-        if (tokens <= 1)
-            r[i]->tok = 0;
-        if (r[i]->heads <= 1)
-            r[i]->head = 0;
         const long long t = r[i]->tok * (tokens - 1), h = r[i]->head * (r[i]->heads - 1), at = i ? apart : 0;
         head_lo[i] = at + std::min(h, 0ll), head_hi[i] = at + std::max(h, 0ll) + r[i]->bytes;
         lo[i] = head_lo[i] + std::min(t, 0ll), hi[i] = head_hi[i] + std::max(t, 0ll);
@@ -381,7 +385,7 @@ int attend(petb200_ctx *ctx, int dtype, PagedArgs a, const int *prefix_table, in
 }
 
 int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *cache, const petb200_kv_seqs *seqs, const int *prefix_table,
-                  int prefix_len, const petb200_kv_rows *q, const petb200_kv_rows *out, int q_heads, int causal, float scale, void *workspace,
+                  int prefix_len, const petb200_kv_rows *q_rows, const petb200_kv_rows *out_rows, int q_heads, int causal, float scale, void *workspace,
                   size_t workspace_bytes, cudaStream_t s) {
     if (!ctx)
         return PETB200_ERR_INVALID;
@@ -393,19 +397,20 @@ int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *ca
         return fail(ctx, PETB200_ERR_INVALID, "%s: the scale must be positive, finite and not denormal", what);
     if (seqs->seqs == 0 || seqs->tokens == 0)
         return PETB200_OK;
-    if (!q || !out || !q->p || !out->p || (prefix_len > 0 && !prefix_table))
+    const petb200_kv_rows q = plain_strides(q_rows, seqs->tokens, q_heads), out = plain_strides(out_rows, seqs->tokens, q_heads);
+    if (!q.p || !out.p || (prefix_len > 0 && !prefix_table))
         return fail(ctx, PETB200_ERR_INVALID, "%s: null argument", what);
     const long long e = 16 / type_size(cache->dtype);
-    if (!on_grid(q->p) || !on_grid(out->p) || q->tok % e || q->head % e || out->tok % e || out->head % e || q->tok < 0 || q->head < 0 || out->tok < 0 || out->head < 0)
+    if (!on_grid(q.p) || !on_grid(out.p) || q.tok % e || q.head % e || out.tok % e || out.head % e || q.tok < 0 || q.head < 0 || out.tok < 0 || out.head < 0)
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q and out must start on 16-byte boundaries", what);
-    if (rows_overlap(*q, q_heads, cache->dtype, *out, q_heads, cache->dtype, cache->dim, seqs->tokens))
+    if (rows_overlap(q, q_heads, cache->dtype, out, q_heads, cache->dtype, cache->dim, seqs->tokens))
         return fail(ctx, PETB200_ERR_INVALID, "%s: out must not overlap q", what);
     if (!on_grid(workspace))
         return fail(ctx, PETB200_ERR_INVALID, "%s: the workspace must be 16-byte aligned", what);
     DeviceGuard guard(ctx->device);
     PagedArgs a = attention_args(ctx, cache, seqs, q_heads);
-    a.q = q->p, a.q_tok = q->tok, a.q_head = q->head;
-    a.out = out->p, a.o_tok = out->tok, a.o_head = out->head;
+    a.q = q.p, a.q_tok = q.tok, a.q_head = q.head;
+    a.out = out.p, a.o_tok = out.tok, a.o_head = out.head;
     a.causal = causal != 0;
     a.sl2 = scale * 1.44269504088896340736f; // log2(e)
     size_t need = 0;
@@ -431,8 +436,9 @@ extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *c
         rotary = 0;
     if (rotary < 0 || rotary > cache->dim || rotary % 2)
         return fail(ctx, PETB200_ERR_INVALID, "%s: %d values of %d cannot be turned in pairs", what, rotary, cache->dim);
-    const petb200_kv_rows none{};
-    const petb200_kv_rows src[3] = {q ? *q : none, k ? *k : none, v ? *v : none}, to = q_out ? *q_out : none;
+    const int tokens = seqs->tokens;
+    const petb200_kv_rows src[3] = {plain_strides(q, tokens, q_heads), plain_strides(k, tokens, cache->heads), plain_strides(v, tokens, cache->heads)};
+    const petb200_kv_rows to = plain_strides(q_out, tokens, q_heads);
     const bool with_q = src[0].p != nullptr;
     if (q_heads < 0 || (with_q && q_heads == 0))
         return fail(ctx, PETB200_ERR_INVALID, "%s: %d query heads", what, q_heads);
@@ -444,7 +450,7 @@ extern "C" int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *c
     if (with_q && (!on_grid(to.p) || to.tok % e || to.head % e || to.tok < 0 || to.head < 0))
         return fail(ctx, PETB200_ERR_UNSUPPORTED, "%s: rows of q_out must start on 16-byte boundaries", what);
     for (int i = 0; with_q && i < 3; ++i)
-        if (rows_overlap(src[i], i ? cache->heads : q_heads, src_dtype, to, q_heads, cache->dtype, cache->dim, seqs->tokens))
+        if (rows_overlap(src[i], i ? cache->heads : q_heads, src_dtype, to, q_heads, cache->dtype, cache->dim, tokens))
             return fail(ctx, PETB200_ERR_INVALID, "%s: q_out must not overlap a source", what);
     AppendArgs a{};
     a.s = device_seqs(ctx, cache, seqs);

@@ -174,3 +174,22 @@ def test_starts_that_claim_more_rows_than_there_are(ctx, dtype, new, keys, group
     assert "q_starts" in told(ctx)
     assert told(ctx) == ""
     c.check(c.attend(ctx))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strides_of_a_single_token_or_head_are_never_used(ctx, dtype):
+    c = Case(dtype, [1], [50], 2, 2, 64, device="cuda", starts=False)
+    k, v, t, n = arguments(c)
+    q, out, q_out = (torch.zeros(256, device="cuda", dtype=dtype).as_strided((1, 4, 64), (257, 64, 1)) for _ in range(3))
+    q.copy_(c.on(c.q))
+    assert ctx.attention_paged(q, k, v, t, n, out=out).data_ptr() == out.data_ptr()
+    c.check(out)
+    ctx.kv_append(q[:, :2], q[:, 2:], k, v, t, n, q=q, q_out=q_out)
+    ctx.sync_check()
+    assert torch.equal(q_out, q) and torch.equal(k[c.table[0, 3].long(), 1], q[0, :2])
+    c = Case(dtype, [3, 3], [50, 60], 1, 1, 64, device="cuda", starts=False)
+    k, v, t, n = arguments(c)
+    q, out = (torch.zeros(6, 64, device="cuda", dtype=dtype).as_strided((6, 1, 64), (64, 3, 1)) for _ in range(2))
+    q.copy_(c.on(c.q))
+    c.check(ctx.attention_paged(q, k, v, t, n, out=out))
+    ctx.sync_check()
