@@ -596,6 +596,8 @@ class Context:
             q_rows, out_rows = L.KV_ROWS.pack(q.data_ptr(), sq[0], sq[1]), L.KV_ROWS.pack(q_out.data_ptr(), so[0], so[1])
         elif q_out is not None:
             raise L.PetError(L.ERR_INVALID, "q_out without q")
+        if not -2 ** 31 <= pos0 < 2 ** 31:
+            raise L.PetError(L.ERR_INVALID, f"pos0: a position of 32 bits expected, got {pos0}")
         pairs, freq = 0, None
         if inv_freq is not None:
             if inv_freq.dtype is not _float32 or inv_freq.dim() != 1 or inv_freq.get_device() != self._kv_device:

@@ -106,3 +106,13 @@ def test_descriptors_are_packed_as_the_header_lays_them_out(tmp_path):
         blob = packed.pack(*values)
         for v, o in zip(values, offsets):
             assert blob[o] == v and blob[o + 1] == 0
+
+
+@pytest.mark.parametrize("pos0", [2 ** 31, -2 ** 31 - 1, 2 ** 40])
+def test_append_refuses_positions_past_32_bits(ctx, pos0):
+    """They would reach the library cut to 32 bits, and turn the keys by other angles."""
+    a = args()
+    q = a.pop("q")
+    with pytest.raises(L.PetError) as e:
+        ctx.kv_append(k=q[:, :2], v=q[:, 2:], inv_freq=torch.ones(32), pos0=pos0, **a)
+    assert e.value.status == L.ERR_INVALID
