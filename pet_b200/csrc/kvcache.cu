@@ -393,8 +393,9 @@ int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *ca
         return rc;
     if (q_heads <= 0 || q_heads % cache->heads)
         return fail(ctx, PETB200_ERR_INVALID, "%s: %d query heads on %d key heads", what, q_heads, cache->heads);
-    if (!std::isfinite(scale) || scale < FLT_MIN)
-        return fail(ctx, PETB200_ERR_INVALID, "%s: the scale must be positive, finite and not denormal", what);
+    const float sl2 = scale * 1.44269504088896340736f; // log2(e)
+    if (!std::isfinite(sl2) || scale < FLT_MIN)
+        return fail(ctx, PETB200_ERR_INVALID, "%s: the scale must be positive, finite (its product with log2(e) too) and not denormal", what);
     if (seqs->seqs == 0 || seqs->tokens == 0)
         return PETB200_OK;
     const petb200_kv_rows q = plain_strides(q_rows, seqs->tokens, q_heads), out = plain_strides(out_rows, seqs->tokens, q_heads);
@@ -412,7 +413,7 @@ int attention_run(petb200_ctx *ctx, const char *what, const petb200_kv_cache *ca
     a.q = q.p, a.q_tok = q.tok, a.q_head = q.head;
     a.out = out.p, a.o_tok = out.tok, a.o_head = out.head;
     a.causal = causal != 0;
-    a.sl2 = scale * 1.44269504088896340736f; // log2(e)
+    a.sl2 = sl2;
     size_t need = 0;
     return attend(ctx, cache->dtype, a, prefix_table, prefix_len, (char *)workspace, workspace ? workspace_bytes : 0, &need, s);
 }

@@ -193,3 +193,18 @@ def test_strides_of_a_single_token_or_head_are_never_used(ctx, dtype):
     q.copy_(c.on(c.q))
     c.check(ctx.attention_paged(q, k, v, t, n, out=out))
     ctx.sync_check()
+
+
+def test_scales_past_what_powers_of_two_hold_are_refused(ctx):
+    """3e38 is finite, its product with log2(e) is not: every score of 0 would be 0 x infinity."""
+    c = Case(F32, [1], [50], 2, 2, 64, device="cuda", starts=False)
+    c.q *= 1e-38
+    for scale in (3e38, 2.4e38):
+        with pytest.raises(PetError) as e:
+            c.attend(ctx, scale=scale)
+        assert e.value.status == ERR_INVALID
+    c.q[:], c.k[:] = 0, 0
+    got = c.attend(ctx, scale=2.3e38).double().cpu()  # all scores are 0: the mean of v
+    want = c.keys(0, c.v).mean(0).repeat_interleave(2, 0)
+    assert ((got[0] - want).abs() <= c.keys(0, c.v).abs().mean(0).repeat_interleave(2, 0) * 2.0 ** -18).all()
+    ctx.sync_check()
