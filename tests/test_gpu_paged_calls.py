@@ -208,3 +208,69 @@ def test_scales_past_what_powers_of_two_hold_are_refused(ctx):
     want = c.keys(0, c.v).mean(0).repeat_interleave(2, 0)
     assert ((got[0] - want).abs() <= c.keys(0, c.v).abs().mean(0).repeat_interleave(2, 0) * 2.0 ** -18).all()
     ctx.sync_check()
+
+
+# ---- routes that a call takes by its sizes ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+# a token of one and of several sequences, a few rows, a prompt; tables of 512 to 131072 keys
+@pytest.mark.parametrize("new,lens,group", [([1], [1500], 4), ([1] * 24, [1 + 60 * b for b in range(24)], 4), ([4, 1], [1500, 3], 2), ([200], [700], 2)])
+@pytest.mark.parametrize("width", [128, 4096])
+def test_tables_much_wider_than_their_sequences(ctx, dtype, new, lens, group, width):
+    c = Case(dtype, new, lens, 2, group, 64, 16, width=width, device="cuda", behind=1)
+    out = torch.full_like(c.q, 5.0).cuda()
+    c.check(c.attend(ctx, out=out))
+    assert (out[c.starts[-1]:] == 5).all()
+    ctx.sync_check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+# the prompt's rows go to 16-row tiles with the tokens, the tokens to the prompt's tiles
+@pytest.mark.parametrize("singles,prompt", [(63, 200), (7, 600)])
+@pytest.mark.parametrize("prefix", [0, 500])
+def test_single_tokens_beside_a_prompt(ctx, dtype, singles, prompt, prefix):
+    new = [1] * (singles // 2) + [prompt] + [1] * (singles - singles // 2)
+    c = Case(dtype, new, [n + 37 * b % 900 for b, n in enumerate(new)], 1, 4, 64, 16, prefix=prefix, device="cuda", behind=2)
+    out = torch.full_like(c.q, 5.0).cuda()
+    c.check(c.attend(ctx, out=out))
+    assert (out[c.starts[-1]:] == 5).all()
+    ctx.sync_check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("starts", [True, False])
+# rows of a sequence that go together with the others' against the shared keys: up to 191, and the first that go alone
+@pytest.mark.parametrize("new,group,prefix", [(1, 4, 3000), (10, 4, 3000), (31, 2, 3000), (31, 2, 2950), (95, 2, 9300), (96, 2, 9300)])
+def test_a_prefix_in_tiles_for_all_sequences(ctx, dtype, dim, starts, new, group, prefix):
+    """The shared keys by TMA (pages that are boxes of a tile), in tiles that hold several sequences' rows."""
+    c = Case(dtype, [new] * 20 if new < 90 else [new] * 3, [new + 9 * b for b in range(20 if new < 90 else 3)], 1, group, dim, 32, prefix=prefix, device="cuda", starts=starts)
+    c.check(c.attend(ctx))
+    ctx.sync_check()
+
+
+@pytest.mark.parametrize("new,group", [(1, 1), (4, 1), (2, 2), (1, 3), (1, 4)])
+@pytest.mark.parametrize("dim", [8, 64, 104, 128])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+def test_infinities_in_few_rows_of_full_precision(ctx, new, group, dim, bad):
+    """Up to four rows of fp32, the newest key infinite: the row that sees it has what the 64-bit form has, the rows before it are as without it."""
+    c = Case(F32, [new] * 5, [max(n, new) for n in (5, 8, 33, 130, 700)], 2, group, dim, 16, device="cuda", starts=False)
+    c.q[:, :, 2] = c.q[:, :, 2].abs() + 0.5
+    want, tol = c.want()
+    for b in range(5):
+        at = c.lens[b] - 1
+        page, slot = c.table[b, at // c.page].long(), at % c.page
+        c.v[page, slot, 1, 3], c.k[page, slot, 0, 2] = bad, bad
+    got = c.attend(ctx).double().cpu()
+    ctx.sync_check()
+    last = torch.zeros(c.tokens, dtype=torch.bool)
+    last[[n - 1 for n in c.starts[1:]]] = True
+    assert ((got - want).abs() <= tol)[~last].all()
+    assert (got[last][:, group:, 3] == bad).all()
+    keep = [d for d in range(dim) if d != 3]
+    assert ((got - want).abs() <= tol)[last][:, group:][:, :, keep].all()
+    if bad > 0:
+        assert torch.isnan(got[last][:, :group]).all()  # inf - inf
+    else:  # weighs nothing: the same queries without their newest key
+        c.lens = [n - 1 for n in c.lens]
+        want, tol = c.want(causal=False)
+        assert ((got - want).abs() <= tol)[last][:, :group].all()
