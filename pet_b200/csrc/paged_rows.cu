@@ -515,10 +515,7 @@ template <int DP, int RR> struct FewRows {
     }
 };
 
-// {m, l, O} of one row from several places, in the order of the pieces.
-struct Joined {
-    float M = -INFINITY, L = 0.f;
-};
+// What a piece's sums are scaled by beside the largest of all pieces' m.
 __device__ __forceinline__ float piece_weight(float m, float M) { return m == -INFINITY ? 0.f : exp2_approx(m - M); }
 
 template <typename T> __device__ __forceinline__ void store4(T *p, float4 v) {
@@ -1017,10 +1014,11 @@ int rows_launch(petb200_ctx *ctx, PagedArgs a, char *ws, size_t ws_bytes, size_t
 
 template <typename T, int DP> int join_launch(petb200_ctx *ctx, const PagedArgs &a, cudaStream_t s) {
     const long long rows = (long long)a.s.tokens * a.group * a.hkv;
-    if (a.pieces <= 4)
+    if (a.pieces <= 4) {
         launch_pdl(k_paged_join_four<T, DP>, dim3((unsigned)((rows + 7) / 8)), 256, 0, s, a);
-    else
-        launch_pdl(k_paged_join_rows<T, DP>, dim3((unsigned)((rows + 3) / 4)), 256, 0, s, a);
+        return launched(ctx, "k_paged_join_four");
+    }
+    launch_pdl(k_paged_join_rows<T, DP>, dim3((unsigned)((rows + 3) / 4)), 256, 0, s, a);
     return launched(ctx, "k_paged_join_rows");
 }
 
