@@ -336,9 +336,12 @@ PagedArgs attention_args(petb200_ctx *ctx, const petb200_kv_cache *cache, const 
 // 64 rows 147 / 68; 32 sequences of 700 keys: 33 / 36, 49 / 36, 67 / 36.
 constexpr int kTileFrom = 17;
 // Rows from which a sequence behind a shared prefix reads it by itself: a row for every 48 shared keys, at most 192.  Rows that go together
-// fill their tiles but meet their own keys in 16-row tiles; alone a sequence's tile is part empty for all of the prefix.  us together /
-// alone: 16 sequences behind 4000 keys, 40 own: 24 rows 37 / 65, 64 rows 57 / 66, 128 rows 74 / 67; 8 behind 16000: 128 rows 106 / 126; 32
-// behind 1000, 300 own: 24 rows 63 / 55, 64 rows 77 / 55.
+// fill their tiles but meet their own keys in 16-row tiles; alone a sequence's tile is part empty for all of the prefix.  fp16, us
+// together / alone, width 128: 16 sequences behind 4000 keys, 20 own beside the new ones: 48 rows 57 / 74, 96 rows 66 / 74, 128 rows 84 / 74; 16
+// behind 8200: 128 rows 117 / 135, 168 rows 184 / 146; 8 behind 16000: 168 rows 129 / 148, 192 rows 131 / 148, 240 rows 176 / 150; 32 behind
+// 1000: 24 rows 57 / 51.  Width 64: 16 behind 4000: 48 rows 41 / 39, 128 rows 57 / 39; 16 behind 8200: 96 rows 55 / 61, 128 rows 70 / 61, 168
+// rows 70 / 72, 192 rows 72 / 74, 240 rows 94 / 74; 8 behind 16000: 128 rows 57 / 59, 168 rows 92 / 70.  What goes together moves in steps, as
+// the tiles of all rows fill the GPU once or twice, so no one border is right everywhere: near it the rule loses up to a quarter.
 long long alone_from(int prefix_len) { return std::min(192, std::max(kTileFrom, prefix_len / 48)); }
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }

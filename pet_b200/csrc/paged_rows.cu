@@ -6,18 +6,21 @@
 // is four warps; a step of it is 4 x CK keys, CK of them (16 halves, 8 floats) per warp, and every warp runs by itself: its
 // own ring of stages filled by its own 16-byte asynchronous copies, its own running maximum, sum and 16 x DP accumulators in
 // registers.  The warps meet once, at the end of a tile.  Bound by HBM: per 16 keys of width 128 a warp issues 32
-// mma.sync.m16n8k16 and 16 ldmatrix beside 8 KB of loads, a third of the issue slots that those 8 KB take to arrive.  (A 16-row tile
+// mma.sync.m16n8k16 and 16 ldmatrix beside 8 KB of loads; 48 % of the issue slots are used over a whole call.  (A 16-row tile
 // would leave seven eighths of a 128-row tcgen05 tile empty; paged_tiles.cu takes over where there are rows for it.)
 //
 // Work is split by ranges: the key steps of all (sequence, row tile, key head) units are laid end to end and every CTA takes an
 // equal share, whatever the lengths; a unit that crosses a border leaves one piece per CTA, and k_paged_join adds the pieces in order.
 // Few units of moderate length go to a thread-block cluster each instead, which adds its sums through shared memory; many units, or
-// units of a few steps, to a CTA each.  64 sequences of up to 8000 keys (1.05 GB): 182 us, 5.8 TB/s; one token on 1500 keys: 11 us a call.
+// units of a few steps, to a CTA each.  64 sequences of up to 8000 keys (1.05 GB): 182 to 188 us,
+// 5.6 to 5.8 TB/s; one token on 1500 keys: 11 us a call.
 //
-// fp32 runs on the TF32 tensor cores (up to four rows: on multiply-adds, see FewRows) with both operands split in two (x = hi + lo, hi the upper 11 bits: hi hi + hi lo + lo hi,
-// 2^-21 of a product left out), and the product with V starts from zero for every 8 keys and is added in registers, since a tensor core's
-// own accumulation cuts off instead of rounding.  Scores, statistics and sums are fp32 for every type; probabilities are
-// rounded to the cache's type for the second product (16-bit types; the sum of the row takes them unrounded).
+// fp32 runs on the TF32 tensor cores (up to four rows: on multiply-adds, see FewRows) with both operands split in two (x = hi + lo, hi the
+// upper 11 bits: hi hi + hi lo + lo hi, 2^-21 of a product left out), and the product with V starts from zero for every 8 keys and is added
+// in registers, since a tensor core's own accumulation cuts off instead of rounding.  Scores, statistics and sums are fp32 for every type;
+// probabilities are rounded to the cache's type for the second product (16-bit types; the sum of the row takes them unrounded).  Prompts
+// in fp32 fetch and split their keys again for every 16 rows: 2000 tokens x 12 heads of 64 take 343 us and 11 of joining, the tensor pipe
+// 25 % busy and 41 % of the issue slots used (629 instructions of a warp per 8 keys, 48 of them products).
 //
 // Rows that see no key give zeros.  A masked key never contributes, whatever its value: its score is replaced before the
 // maximum, and non-finite values of its v are taken out of the stage before the product (see `scrub`).  Infinities that are seen give what
@@ -404,8 +407,8 @@ template <typename T, int DP> struct RowTile {
 };
 
 // The same for up to RR rows in fp32 by multiply-adds: a tensor-core tile would be mostly empty, and splitting K and V in two for it is
-// what it spends its time on (one row of width 64: 420 instructions per 8 keys, 105 here).  LPK lanes share a key, four values of it
-// each; with width 64 the warp has two keys at a time.  Products and sums are plain fp32.
+// what it spends its time on (16 sequences of up to 1100 keys, one row of each of 12 heads of 64: 38 us a call in tiles, 25 this way).  LPK
+// lanes share a key, four values of it each; with width 64 the warp has two keys at a time.  Products and sums are plain fp32.
 template <int DP, int RR> struct FewRows {
     using C = RowCfg<float, DP>;
     static constexpr int LPK = DP / 4, KPP = 32 / LPK, NP = C::CK / KPP, QR = RR * 4;

@@ -15,9 +15,9 @@
 // two products (1270).  Tried and no faster: part of the powers as polynomials on the FMA pipe (more instructions), two threads a row,
 // quarters of a tile in a rolled loop, the maximum of the tile before taken first and checked beside the powers, and blocks that
 // stay and take unit after unit (registers spilled).  Beside the keys a unit costs 11 k cycles until its first scores and 5 k for its
-// results.  500 tokens x 16 heads on 33 k keys: 149 us, 900 TFLOP/s; tensor pipe busy 58 % (profiles/paged_attention.md).
+// results.  500 tokens x 16 heads on 33 k keys: 149 to 151 us, 890 TFLOP/s; tensor pipe busy 58 % (profiles/paged_attention.md).
 // The maximum moves only where a row's grows by more than 2^8 over the one in use (then O and l are scaled, by the softmax warps): the
-// sums stay within range and any m gives the same quotient.
+// sums stay within range and any m gives the same quotient.  fp16 takes the maximum less 7 (see lifted()).
 //
 // K and V tiles are fetched by TMA, a box per page (or part of a page) and 64 columns, in the 128-byte swizzle (16-byte piece c of row r at
 // c ^ (r & 7)); V is the second product's B operand as it lies, its rows along K ("MN-major").  Pages that do not fit the tiles (a
