@@ -274,3 +274,97 @@ def test_infinities_in_few_rows_of_full_precision(ctx, new, group, dim, bad):
         c.lens = [n - 1 for n in c.lens]
         want, tol = c.want(causal=False)
         assert ((got - want).abs() <= tol)[last][:, :group].all()
+
+
+# ---- more of what the documentation allows --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new,lens,prefix", [([2, 0, 3], [60, 9, 700], 0), ([40, 70], [90, 300], 0), ([1, 2, 1], [7, 40, 20], 900), ([30, 60], [30, 300], 900)])
+def test_rows_before_the_first_sequence_are_left_alone(ctx, dtype, new, lens, prefix):
+    c = Case(dtype, new, lens, 2, 3, 64, 16, prefix=prefix, device="cuda")
+    k, v, t, n = arguments(c)
+    q, out = (torch.full((c.tokens + 5, 6, 64), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+    q[3:-2] = c.on(c.q)
+    starts = c.on(c.q_starts) + 3
+    if prefix:
+        ctx.attention_prefix(q, k, v, c.on(c.prefix_table), prefix, t, n, q_starts=starts, out=out)
+    else:
+        ctx.attention_paged(q, k, v, t, n, q_starts=starts, out=out)
+    c.check(out[3:-2])
+    assert (out[:3] == 7).all() and (out[-2:] == 7).all()
+    before, out = (k.clone(), v.clone()), torch.full_like(q, 5.0)
+    ctx.kv_append(q[:, :2], q[:, 2:4], k, v, t, n, q_starts=starts, q=q, q_out=out)
+    ctx.sync_check()
+    assert torch.equal(out[3:-2], q[3:-2]) and (out[:3] == 5).all() and (out[-2:] == 5).all()
+    changed = sum(min(a, b) for a, b in zip(new, lens))
+    assert int(((k != before[0]) & ~(k.isnan() & before[0].isnan())).flatten(2).any(2).sum()) == changed
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new", [1, 60])
+def test_pages_that_several_sequences_share(ctx, dtype, new):
+    """Samples of one question: the same pages in several rows of the table, and one page twice in a row."""
+    c = Case(dtype, [new] * 4, [200 + b for b in range(4)], 2, 2, 64, 16, device="cuda", garbage=False)
+    c.table[1:, :10] = c.table[0, :10]
+    c.table[2, 3] = c.table[2, 7]
+    c.check(c.attend(ctx))
+    ctx.sync_check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("group,dim", [(64, 64), (128, 128), (300, 40)])
+def test_very_many_query_heads_on_one_key_head(ctx, dtype, group, dim):
+    c = Case(dtype, [1, 2, 1], [900, 40, 1], 1, group, dim, 16, device="cuda")
+    c.check(c.attend(ctx))
+    c = Case(dtype, [1] * 4, [70, 3, 1, 33], 1, group, dim, 16, prefix=300, device="cuda", starts=False)
+    c.check(c.attend(ctx))
+    ctx.sync_check()
+
+
+def test_a_first_call_inside_a_capture():
+    """A context whose kernels have never run: limits are raised and tensor maps encoded while the stream is captured."""
+    from pet_b200.ops import Context
+    fresh = Context(0)
+    cases = [Case(BF16, [1] * 3, [50, 1, 200], 2, 4, 64, device="cuda", starts=False), Case(F16, [150], [700], 1, 2, 128, device="cuda"),
+             Case(F32, [1] * 40, [300] * 40, 2, 2, 128, device="cuda", starts=False), Case(BF16, [1] * 40, [30] * 40, 2, 4, 64, prefix=2000, device="cuda")]
+    args = [(c.on(c.q), *arguments(c), c.on(c.q_starts), c.on(c.prefix_table)) for c in cases]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = [fresh.attention_prefix(q, k, v, p, c.prefix, t, n, q_starts=s) if c.prefix else fresh.attention_paged(q, k, v, t, n, q_starts=s)
+               for c, (q, k, v, t, n, s, p) in zip(cases, args)]
+    for _ in range(2):
+        graph.replay()
+    fresh.sync_check()
+    for c, y in zip(cases, got):
+        c.check(y)
+    del graph
+    fresh.close()
+
+
+def test_workspaces_of_the_library_are_checked(ctx):
+    """The C entry points with no workspace, one that is a byte short, one off the grid: refused, and nothing is written."""
+    import ctypes as C
+    from pet_b200 import lib as L
+    lib = L.load()
+    for c in (Case(F32, [1] * 40, [3000] * 40, 2, 2, 64, device="cuda", starts=False), Case(BF16, [100], [9000], 1, 1, 64, device="cuda", starts=False),
+              Case(BF16, [1] * 40, [30] * 40, 2, 4, 64, prefix=2000, device="cuda", starts=False), Case(BF16, [1] * 3, [30] * 3, 2, 4, 64, prefix=900, device="cuda", starts=False)):
+        k, v, t, n = arguments(c)
+        q, p = c.on(c.q), c.on(c.prefix_table)
+        out = torch.full_like(q, 3.0)
+        cache, seqs, *_ = ctx._kv_call(c.tokens, k, v, t, n, None)
+        heads, need = q.shape[1], C.c_size_t()
+        rows = [L.KV_ROWS.pack(x.data_ptr(), x.stride(0), x.stride(1)) for x in (q, out)]
+        assert lib.petb200_attention_paged_workspace(ctx.h, cache, seqs, c.prefix, heads, C.byref(need)) == 0 and need.value > 0
+        work = torch.empty(need.value + 16, dtype=torch.uint8, device="cuda")
+
+        def run(at, size):
+            stream = torch.cuda.current_stream().cuda_stream
+            if c.prefix:
+                return lib.petb200_attention_prefix_run(ctx.h, cache, seqs, p.data_ptr(), c.prefix, *rows, heads, 1, c.dim ** -0.5, at, size, stream)
+            return lib.petb200_attention_paged_run(ctx.h, cache, seqs, *rows, heads, 1, c.dim ** -0.5, at, size, stream)
+        for at, size in ((None, 0), (None, need.value), (work.data_ptr(), need.value - 1), (work.data_ptr() + 8, need.value)):
+            assert run(at, size) == ERR_INVALID
+        ctx.sync_check()
+        assert (out == 3).all()
+        assert run(work.data_ptr(), need.value) == 0
+        c.check(out)
+    ctx.sync_check()
