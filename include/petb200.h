@@ -243,7 +243,8 @@ int petb200_kv_append_run(petb200_ctx *ctx, const petb200_kv_cache *cache, const
                           const float *inv_freq, int rotary, int interleaved, int pos0, petb200_stream stream);
 /* out[token, head] = sum_j softmax_j(scale q . k_j) v_j over the token's sequence, query head `head` on key head
  * head / (q_heads / heads).  causal: token i of n sees keys j <= kv_lens[b] - n + i, else all kv_lens[b].  A row that sees no key
- * gives zeros; rows outside all sequences are left as they were; masked and absent keys never contribute, whatever they hold.
+ * gives zeros; rows outside all sequences are left as they were; masked and absent keys never contribute, whatever they hold.  Infinities
+ * that are seen give what the formula gives (infinity or NaN where their probability rounds to zero).
  * q and out are of the cache's type, rows 16-byte aligned, and must not overlap (PETB200_ERR_INVALID), nor out the pools.  Scores, softmax and
  * sums are fp32 (F32 caches: products error-compensated TF32; 16-bit caches: probabilities rounded to the cache's type).  `workspace` is device memory of the size that
  * petb200_attention_paged_workspace gives for the same call (prefix_len 0), used until the launches have run. */
